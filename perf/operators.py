@@ -189,8 +189,8 @@ def prepare(case, seed):
     else:
         n = case["n"]
         s["a"] = _stored(_rows(g, rows, k), case["bits"])
-        if op == "glu":          # strips of 32 gate rows and their 32 up rows, the last strip filled with zero rows
-            pad = _up(n, BLOCK) - n
+        if op == "glu":          # strips of 32 gate rows and their 32 up rows, whole chunks of columns with zero rows
+            pad = _up(n, CHUNK) - n
             both = [torch.nn.functional.pad(_weights(g, n, k), (0, 0, 0, pad)).view(-1, BLOCK, k) for _ in range(2)]
             s["w"] = _stored(torch.stack(both, dim=1).view(-1, k), 4)
         else:
@@ -212,7 +212,7 @@ def _run_own(s):
     if op == "norm":
         h = ops.mx_rmsnorm(s["x"], s["weight"], 1e-6, bits=8, delta=s["delta_rows"])
         return s["x"], ops.mx_dequantize(h)
-    a, w = MxRows(*s["a"], s["bits"], s["k"]), MxRows(*s["w"], 4, s["k"])
+    a, w = MxRows(*s["a"], s["bits"], s["k"]), MxRows(*s["w"], 4, s["k"], settled=True)
     if op == "glu":
         return ops.mx_dequantize(ops.mx_linear_glu(a, w, s["n"], bits=8))
     ops.mx_linear(a, w, s["out"], accumulate=s["add"])

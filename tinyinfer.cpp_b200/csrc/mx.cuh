@@ -1,0 +1,110 @@
+// The microscaled format and the tensor-core instructions that read it.
+//
+// A row is cut into blocks of 32 elements.  A block has one scale byte s that stands for 2^(s - 127) (255: NaN), an element
+// is e2m1 (4 bits: 0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives) or e4m3 (8 bits, up to 448).  With E the biased binary
+// exponent of the block's largest magnitude, s = max(E - emax, 0) with emax = 2 or 8, the exponent of the element type's
+// largest power of two; elements are rounded to nearest even and saturate.  A block with an infinity or a NaN has s = 255:
+// its row's products are NaN and not some finite number.
+//
+// In memory rows are padded with zeros to whole chunks of 128 elements (so that a row of operands for the tensor cores, 128
+// bytes of 4-bit codes unpacked or of 8-bit codes, never ends inside), two 4-bit codes share a byte, the even element low.
+// The scales of 128 rows and one chunk are 512 bytes, [row % 32][row / 32 % 4][block % 4], the tiles of a row's chunks one
+// behind the other: one tcgen05.cp of 32 rows of 128 bits brings such a tile into four columns of tensor memory, the form in
+// which the block-scaled products want it.  Rows up to the next multiple of 128 have scale bytes that nothing depends on.
+#pragma once
+
+#include "sm100.cuh"
+
+namespace mx {
+
+constexpr int BLOCK = 32, CHUNK = 128, TILE_ROWS = 128, TILE_BYTES = 512;
+
+// where the scale byte of (row, block) lies; `chunks` = padded row length / 128
+__host__ __device__ __forceinline__ size_t scale_at(int row, int block, int chunks) {
+    return ((size_t)(row / TILE_ROWS) * chunks + block / 4) * TILE_BYTES + (row % 32) * 16 + (row / 32 % 4) * 4 + block % 4;
+}
+
+template <int BITS> constexpr int EMAX = BITS == 4 ? 2 : 8;
+
+// the scale byte of a block whose largest magnitude has these float32 bits (sign removed)
+template <int BITS> __device__ __forceinline__ unsigned scale_byte(unsigned top) {
+    const int e = (int)(top >> 23);
+    return e == 255 ? 255u : (unsigned)max(e - EMAX<BITS>, 0);
+}
+// 2^(127 - s), what elements are multiplied by; a product with a power of two is exact.  s <= 254 - emax, so the result is
+// normal; s = 255 gives 0 (the codes then do not matter)
+__device__ __forceinline__ float scale_inverse(unsigned s) { return s == 255 ? 0.0f : __uint_as_float((254u - s) << 23); }
+// 2^(s - 127)
+__device__ __forceinline__ float scale_value(unsigned s) {
+    return __uint_as_float(s == 255 ? 0x7fffffffu : s == 0 ? 0x00400000u : s << 23);
+}
+
+// two neighbours' codes: e4m3 in the low 16 bits, e2m1 in the low 8 (the first element low)
+__device__ __forceinline__ unsigned codes_e4m3x2(float first, float second) {
+    unsigned short r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(second), "f"(first));
+    return r;
+}
+__device__ __forceinline__ unsigned codes_e2m1x2(float first, float second) {
+    unsigned r;
+    asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\tcvt.u32.u8 %0, b;\n\t}" : "=r"(r) : "f"(second), "f"(first));
+    return r;
+}
+// the value of one code
+__device__ __forceinline__ float value_e4m3(unsigned c) {
+    // exponent and mantissa moved to float16's places give value / 2^8; e = 15 with mantissa 7 is NaN
+    if ((c & 0x7f) == 0x7f) return __uint_as_float(0x7fffffffu);
+    const unsigned mag = c & 0x7f;
+    const float v = mag >= 8 ? __uint_as_float((mag << 20) + (120u << 23)) : (float)mag * 0.001953125f;
+    return c & 0x80 ? -v : v;
+}
+__device__ __forceinline__ float value_e2m1(unsigned c) {
+    const unsigned mag = c & 7;
+    const float v = mag >= 2 ? __uint_as_float((mag << 22) + (126u << 23)) : (float)mag * 0.5f;
+    return c & 8 ? -v : v;
+}
+
+// ---- block-scaled products -----------------------------------------------------------------------
+
+// Descriptor of 32 rows of 16 bytes without a swizzle: groups of 8 rows are 128 bytes apart.
+__device__ __forceinline__ unsigned long long scale_desc(const void* p) {
+    return (unsigned long long)((sm100::smem_u32(p) & 0x3FFFF) >> 4) | (unsigned long long)1 << 16 |
+           (unsigned long long)(128 >> 4) << 32 | (unsigned long long)1 << 46;
+}
+// Instruction descriptor of a block-scaled product with power-of-two scales; the scale bytes of a step of K are chosen in
+// their 32-bit words by `id` (bits 4-5 for B, 29-30 for A).
+__device__ __forceinline__ unsigned scaled_idesc(int m, int n, unsigned a_type, unsigned b_type) {
+    return (a_type << 7) | (b_type << 10) | ((unsigned)(n >> 3) << 17) | (1u << 23) | ((unsigned)(m >> 4) << 24);
+}
+__device__ __forceinline__ unsigned with_ids(unsigned idesc, unsigned id) { return idesc | (id << 4) | (id << 29); }
+
+// element types in the instruction descriptor: with 4-bit operands on both sides e2m1 is 1; in the products of 8-, 6- and
+// 4-bit elements e4m3 is 0 and e2m1 5
+constexpr unsigned FOUR_E2M1 = 1, MIXED_E4M3 = 0, MIXED_E2M1 = 5;
+
+// Contiguous bytes from global to shared memory, counted by the barrier; addresses and size multiples of 16.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, unsigned bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(sm100::smem_u32(dst)), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// codes of `rows` rows of `kp` elements as tiles of box_rows rows x 128 bytes of shared memory with the 128-byte swizzle:
+// packed (`unpack` false; 4-bit: 256 elements, 8-bit: 128), or 4-bit codes spread to a byte's space each (128 elements, every
+// 16 of them 8 bytes followed by 8 bytes of padding), the form of 4-bit elements beside 8-bit ones.  Zeros outside.
+inline int make_map_codes(CUtensorMap* map, const void* base, int rows, int kp, int bits, bool unpack, int box_rows,
+                          const char* who) {
+    sm100::EncodeTiled fn = sm100::encode_fn();
+    if (!fn) return ti_fail("%s: the driver lacks cuTensorMapEncodeTiled", who);
+    const cuuint64_t bytes = (cuuint64_t)kp * bits / 8;
+    const cuuint64_t dims[2] = {unpack ? (cuuint64_t)kp : bytes, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {bytes};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    const cuuint32_t elem[2] = {1, 1};
+    CUresult r = fn(map, unpack ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
+                    const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return ti_fail("%s: cuTensorMapEncodeTiled failed with %d", who, (int)r);
+    return 0;
+}
+
+}  // namespace mx

@@ -1,0 +1,383 @@
+// Products of microscaled rows with 4-bit microscaled weights on block-scaled tcgen05 instructions:
+//   C[M, N] (+)= A[M, K] W[N, K]^T, or codes of silu(A G^T) * (A U^T), sums in float32 in tensor memory.
+//
+// The roles of the operands are swapped: 128 rows of W are the instruction's M side, NTOK rows of A its N side, so a step of
+// few rows streams W once and wastes nothing on empty rows of A.  A stage of the ring is 128 bytes of every operand row: 256
+// elements where both sides have 4 bits, 128 where A has 8 (W's codes then take a byte each in shared memory; the spreading
+// is TMA's), with the scale tiles of those elements beside it.  The MMA thread copies a stage's scale tiles into tensor
+// memory columns of that stage (tcgen05.cp runs in order with the products behind it; columns are written again when the
+// stage's "empty" barrier has seen the products that read them).
+//
+// K is cut over the blocks of a cluster: each keeps its part of the sum in its shared memory, and after a cluster barrier
+// every block adds the parts of its share of the tokens, in the order of the blocks (no atomics: the same bits each run).
+// The number of parts depends on N, K and the tile alone.
+//
+// W's rows for the gated form are strips of 32 gate rows and their 32 up rows: 32 outputs are one warp's lanes and one block
+// of the format.
+//
+// Every wait is bounded; on a timeout the block records status 2 and leaves like the others.
+#include "mx.cuh"
+
+namespace {
+
+using namespace sm100;
+using namespace mx;
+
+constexpr int BW = 128, THREADS = 192;       // TMA warp, MMA warp, four epilogue warps
+constexpr int ROW = 128;                     // bytes of an operand row in a stage
+enum { MODE_STORE = 0, MODE_ACCUMULATE = 1, MODE_GLU = 2 };
+enum { TI_ERR_TIMEOUT = 2 };
+
+template <int NTOK, int ABITS> struct Tile {
+    static constexpr int ELEMS = ABITS == 4 ? 256 : 128;                 // of K in a stage
+    static constexpr int CHUNKS = ELEMS / CHUNK;
+    static constexpr int XTILES = (NTOK + TILE_ROWS - 1) / TILE_ROWS;     // scale tiles of A per chunk
+    static constexpr int STAGE_W = BW * ROW, STAGE_X = NTOK * ROW;
+    static constexpr int STAGE_S = CHUNKS * (1 + XTILES) * TILE_BYTES;
+    static constexpr int PER_SM = NTOK <= 128 ? 2 : 1;                    // blocks of an SM
+    static constexpr int STAGES = NTOK == 256 ? 4 : NTOK == 128 ? 3 : NTOK == 64 ? 4 : 5;
+    static constexpr int SMEM = STAGES * (STAGE_W + STAGE_X + STAGE_S) + 1024 + 256;
+    static constexpr int SCALE_COLS = CHUNKS * 4 * (1 + XTILES);          // tensor memory columns of a stage's scales
+    static constexpr int ACC_COLS = NTOK < 32 ? 32 : NTOK;
+    static constexpr int COLS = ACC_COLS + STAGES * SCALE_COLS;
+    static constexpr unsigned TMEM_COLS = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+    static_assert(COLS <= 512 && TMEM_COLS * PER_SM <= 512, "tensor memory");
+    static_assert(SMEM * PER_SM <= 227 * 1024, "shared memory");
+    static_assert(STAGES * (STAGE_W + STAGE_X) >= NTOK * BW * 4, "the sums of a tile have to fit where the stages were");
+};
+
+struct Args {
+    const unsigned char *w_scales, *x_scales;
+    float* c;
+    unsigned char *out_codes, *out_scales;
+    int m, n, kp, ldc, out_kp, mode, parts, tiles_n, settled;
+    int* status;
+};
+
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n" ::: "memory");
+    asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ unsigned map_to_rank(unsigned addr, unsigned rank) {
+    unsigned out;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
+    return out;
+}
+__device__ __forceinline__ float load_cluster(unsigned addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 load_cluster4(unsigned addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void copy_scales(unsigned tmem, const void* tile) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(scale_desc(tile)) : "memory");
+}
+template <int ABITS>
+__device__ __forceinline__ void umma_scaled(unsigned tmem_d, unsigned long long da, unsigned long long db, unsigned idesc,
+                                            unsigned sfa, unsigned sfb, unsigned accumulate) {
+    if (ABITS == 4)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+            ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+            ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+
+// The gated rows of a token's 64 outputs of this tile, summed over the parts, as codes: lanes are the 32 outputs of a block.
+template <int OBITS>
+__device__ __forceinline__ void finish_glu(const Args& p, float gate, float up, int tok, int out_col, int lane) {
+    const float h = up * gate / (1.0f + expf(-gate));
+    const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
+    const unsigned s = scale_byte<OBITS>(top);
+    const float y = h * scale_inverse(s);
+    const size_t el = (size_t)tok * p.out_kp + out_col + lane;
+    if (OBITS == 8) {
+        p.out_codes[el] = (unsigned char)codes_e4m3x2(y, 0.0f);
+    } else {
+        const float next = __shfl_down_sync(0xffffffffu, y, 1);
+        if (!(lane & 1)) p.out_codes[el / 2] = (unsigned char)codes_e2m1x2(y, next);
+    }
+    if (lane == 0) p.out_scales[scale_at(tok, out_col / BLOCK, p.out_kp / CHUNK)] = (unsigned char)s;
+}
+
+template <int NTOK, int ABITS, int OBITS>
+__global__ void __launch_bounds__(THREADS)
+mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Args p) {
+    using T = Tile<NTOK, ABITS>;
+    constexpr int STAGES = T::STAGES, CHUNKS = T::CHUNKS, XTILES = T::XTILES;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char* stage_w = smem;
+    unsigned char* stage_x = smem + STAGES * T::STAGE_W;
+    unsigned char* stage_s = smem + STAGES * (T::STAGE_W + T::STAGE_X);
+    unsigned long long* bars = (unsigned long long*)(stage_s + STAGES * T::STAGE_S);
+    unsigned long long *full = bars, *empty = bars + STAGES, *acc_full = bars + 2 * STAGES;
+    unsigned* tmem_slot = (unsigned*)(bars + 2 * STAGES + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int part = (int)cluster_rank(), unit = (int)blockIdx.x / p.parts;
+    const int n0 = unit % p.tiles_n * BW, tok0 = unit / p.tiles_n * NTOK;
+    const int chunks = p.kp / CHUNK, num_kb = (chunks + CHUNKS - 1) / CHUNKS;
+    const int kb0 = (int)((long long)part * num_kb / p.parts), kb1 = (int)((long long)(part + 1) * num_kb / p.parts);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        mbar_init(acc_full, 1);
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, T::TMEM_COLS);
+    pdl_launch();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem_base = *tmem_slot;
+
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            const int x_tiles = min(XTILES, (p.m - tok0 + TILE_ROWS - 1) / TILE_ROWS);
+            auto stage_bytes = [&](int held) {               // what TMA counts for a stage that holds `held` chunks: spread codes
+                                                             // count as they are packed, half of the space they take
+                return (unsigned)(T::STAGE_W / (ABITS == 8 ? 2 : 1) + T::STAGE_X + held * (1 + x_tiles) * TILE_BYTES);
+            };
+            auto load_w = [&](int kb, int s) {
+                const int held = min(CHUNKS, chunks - kb * CHUNKS);
+                mbar_expect_tx(&full[s], stage_bytes(held));
+                tma_load_2d(stage_w + s * T::STAGE_W, &map_w, &full[s], kb * ROW, n0);
+                bulk_load(stage_s + s * T::STAGE_S, p.w_scales + ((size_t)(n0 / TILE_ROWS) * chunks + kb * CHUNKS) * TILE_BYTES,
+                          (unsigned)(held * TILE_BYTES), smem_u32(&full[s]));
+            };
+            int primed = 0;
+            if (p.settled)                                    // W is older than the kernel in front of this one
+                for (; primed < STAGES && kb0 + primed < kb1; ++primed) load_w(kb0 + primed, primed);
+            pdl_wait();
+            for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+                const int s = it % STAGES;
+                if (it >= primed) {
+                    ok = mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1);
+                    if (!ok) break;
+                    load_w(kb, s);
+                }
+                const int held = min(CHUNKS, chunks - kb * CHUNKS);
+                tma_load_2d(stage_x + s * T::STAGE_X, &map_x, &full[s], kb * ROW, tok0);
+                for (int j = 0; j < x_tiles; ++j)
+                    bulk_load(stage_s + s * T::STAGE_S + CHUNKS * (1 + j) * TILE_BYTES,
+                              p.x_scales + ((size_t)(tok0 / TILE_ROWS + j) * chunks + kb * CHUNKS) * TILE_BYTES,
+                              (unsigned)(held * TILE_BYTES), smem_u32(&full[s]));
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const unsigned idesc = ABITS == 4 ? scaled_idesc(BW, NTOK, FOUR_E2M1, FOUR_E2M1)
+                                              : scaled_idesc(BW, NTOK, MIXED_E2M1, MIXED_E4M3);
+            for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+                const int s = it % STAGES, held = min(CHUNKS, chunks - kb * CHUNKS);
+                ok = mbar_wait(&full[s], (it / STAGES) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const unsigned cols = tmem_base + T::ACC_COLS + s * T::SCALE_COLS;
+                for (int j = 0; j < held; ++j) {              // columns of a chunk: W's four, then four per scale tile of A
+                    copy_scales(cols + j * 4 * (1 + XTILES), stage_s + s * T::STAGE_S + j * TILE_BYTES);
+#pragma unroll
+                    for (int t = 0; t < XTILES; ++t)
+                        copy_scales(cols + j * 4 * (1 + XTILES) + 4 * (1 + t),
+                                    stage_s + s * T::STAGE_S + (CHUNKS * (1 + t) + j) * TILE_BYTES);
+                }
+                const unsigned long long dw = umma_desc(stage_w + s * T::STAGE_W), dx = umma_desc(stage_x + s * T::STAGE_X);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {              // 32 bytes of every row: 64 or 32 elements
+                    const int j = ABITS == 4 ? kk / 2 : 0;
+                    if (j >= held) break;
+                    const unsigned sf = cols + j * 4 * (1 + XTILES);
+                    umma_scaled<ABITS>(tmem_base, dw + kk * 2, dx + kk * 2, with_ids(idesc, ABITS == 4 ? kk % 2 * 2 : kk), sf,
+                                       sf + 4, it > 0 || kk > 0);
+                }
+                umma_commit(&empty[s]);
+            }
+            umma_commit(acc_full);
+        }
+    } else {
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        pdl_wait();                                           // C belongs to the chain of launches
+        ok = mbar_wait(acc_full, 0);
+        tc_fence_after();
+        const unsigned acc = tmem_base + ((unsigned)(quarter * 32) << 16);
+        const int held_tok = min(NTOK, p.m - tok0);
+        if (p.mode != MODE_GLU && p.parts == 1) {             // straight to C: a warp's lanes are 32 neighbouring columns
+#pragma unroll 1
+            for (int t0 = 0; t0 < held_tok; t0 += 16) {
+                float v[16];
+                tmem_load16(acc + t0, v);
+                if (n0 + row < p.n) {
+                    float* dst = p.c + (size_t)(tok0 + t0) * p.ldc + n0 + row;
+                    if (p.mode == MODE_ACCUMULATE) {          // all old values asked for before the first store
+                        float old[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) old[i] = t0 + i < held_tok ? __ldcg(dst + (size_t)i * p.ldc) : 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] += old[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (t0 + i < held_tok) dst[(size_t)i * p.ldc] = v[i];
+                }
+                __syncwarp();
+            }
+        } else {                                              // the sums where the stages were: all products have read them
+            float* sums = (float*)smem;
+#pragma unroll 1
+            for (int t0 = 0; t0 < held_tok; t0 += 16) {
+                float v[16];
+                tmem_load16(acc + t0, v);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sums[(t0 + i) * BW + row] = v[i];
+            }
+        }
+    }
+    if (!ok) atomicCAS(p.status, 0, TI_ERR_TIMEOUT);
+    tc_fence_before();
+    __syncwarp();
+    if (p.mode == MODE_GLU || p.parts > 1) {
+        cluster_sync();
+        const int held_tok = min(NTOK, p.m - tok0);
+        const unsigned sums = smem_u32(smem);
+        pdl_wait();
+        if (p.mode == MODE_GLU) {
+            // (token, strip) pairs of this block's share
+            for (int i = warp; i < (held_tok - part + p.parts - 1) / p.parts * 2; i += THREADS / 32) {
+                const int t = part + i / 2 * p.parts, strip = i & 1;
+                if (n0 + strip * 64 >= p.n) continue;
+                float gate = 0.0f, up = 0.0f;
+                for (int r = 0; r < p.parts; ++r) {
+                    const unsigned at = map_to_rank(sums + (t * BW + strip * 64 + lane) * 4, r);
+                    gate += load_cluster(at);
+                    up += load_cluster(at + 32 * 4);
+                }
+                finish_glu<OBITS>(p, gate, up, tok0 + t, n0 / 2 + strip * 32, lane);
+            }
+        } else {
+            const bool by4 = p.ldc % 4 == 0 && p.n % 4 == 0 && (uintptr_t)p.c % 16 == 0;
+            for (int t = part + warp * p.parts; t < held_tok; t += THREADS / 32 * p.parts) {
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int r = 0; r < p.parts; ++r) {
+                    const float4 o = load_cluster4(map_to_rank(sums + (t * BW + lane * 4) * 4, r));
+                    v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+                }
+                const int col = n0 + lane * 4;
+                float* dst = p.c + (size_t)(tok0 + t) * p.ldc + col;
+                if (by4) {
+                    if (col >= p.n) continue;
+                    if (p.mode == MODE_ACCUMULATE) {
+                        const float4 o = __ldcg(reinterpret_cast<const float4*>(dst));
+                        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+                    }
+                    *reinterpret_cast<float4*>(dst) = v;
+                } else {
+                    const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (col + i < p.n) dst[i] = (p.mode == MODE_ACCUMULATE ? __ldcg(dst + i) : 0.0f) + f[i];
+                }
+            }
+        }
+        cluster_sync();                                       // nobody leaves while its sums may be read
+    } else {
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, T::TMEM_COLS);
+    }
+}
+
+template <int NTOK, int ABITS, int OBITS>
+int launch(const void* w, const void* x, Args p, void* stream) {
+    using T = Tile<NTOK, ABITS>;
+    auto kernel = mx_gemm_kernel<NTOK, ABITS, OBITS>;
+    CUtensorMap map_w, map_x;
+    if (int rc = make_map_codes(&map_w, w, p.n, p.kp, 4, ABITS == 8, BW, "mx_gemm")) return rc;
+    if (int rc = make_map_codes(&map_x, x, p.m, p.kp, ABITS, false, NTOK, "mx_gemm")) return rc;
+    static TiPerDevice configured;
+    if (configured.first_use()) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+        if (e != cudaSuccess) return ti_fail("mx_gemm: %s", cudaGetErrorString(e));
+        configured.mark();
+    }
+    int device = 0, sms = 0;
+    cudaGetDevice(&device);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    p.tiles_n = (p.n + BW - 1) / BW;
+    const int tiles = p.tiles_n * ((p.m + NTOK - 1) / NTOK), num_kb = (p.kp + T::ELEMS - 1) / T::ELEMS;
+    p.parts = 1;
+    while (p.parts < 8 && tiles * p.parts * 2 <= sms * T::PER_SM && p.parts * 2 <= num_kb) p.parts *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = (unsigned)(tiles * p.parts);
+    cfg.blockDim = THREADS;
+    cfg.dynamicSmemBytes = T::SMEM;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.parts;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, (const Args)p);
+    return ti_check_launch("mx_gemm");
+}
+
+template <int ABITS, int OBITS> int launch_rows(const void* w, const void* x, const Args& p, void* stream) {
+    return p.m <= 16 ? launch<16, ABITS, OBITS>(w, x, p, stream) : p.m <= 32 ? launch<32, ABITS, OBITS>(w, x, p, stream)
+         : p.m <= 64 ? launch<64, ABITS, OBITS>(w, x, p, stream) : p.m <= 128 ? launch<128, ABITS, OBITS>(w, x, p, stream)
+         : launch<256, ABITS, OBITS>(w, x, p, stream);
+}
+
+int check(const char* who, const void* a, const void* a_scales, int a_bits, const void* w, const void* w_scales, int m, int n,
+          int kp) {
+    TI_REQUIRE(a_bits == 4 || a_bits == 8, "%s: rows of %d bits (4 and 8 are known)", who, a_bits);
+    TI_REQUIRE(m >= 0 && n >= 0 && kp >= CHUNK && kp % CHUNK == 0, "%s: M=%d, N=%d, padded K=%d", who, m, n, kp);
+    TI_REQUIRE((uintptr_t)a % 32 == 0 && (uintptr_t)w % 32 == 0 && (uintptr_t)a_scales % 16 == 0 &&
+               (uintptr_t)w_scales % 16 == 0, "%s: codes must start on 32 bytes, scales on 16", who);
+    return 0;
+}
+
+}  // namespace
+
+// c[m, n] (+)= a w^T.  a: codes of a_bits, w: codes of 4 bits, rows of kp elements.  settled: nothing in flight writes w.
+extern "C" int ti_mx_gemm(const void* a, const void* a_scales, int a_bits, const void* w, const void* w_scales, float* c, int m,
+                          int n, int kp, int ldc, int accumulate, int settled, int* status, void* stream) {
+    if (int rc = check("mx_gemm", a, a_scales, a_bits, w, w_scales, m, n, kp)) return rc;
+    TI_REQUIRE((uintptr_t)c % 4 == 0 && ldc >= n, "mx_gemm: rows of %d floats for %d columns", ldc, n);
+    if (m == 0 || n == 0) return 0;
+    const Args p{(const unsigned char*)w_scales, (const unsigned char*)a_scales, c, nullptr, nullptr, m, n, kp, ldc, 0,
+                 accumulate ? MODE_ACCUMULATE : MODE_STORE, 1, 0, settled, status};
+    return a_bits == 4 ? launch_rows<4, 8>(w, a, p, stream) : launch_rows<8, 8>(w, a, p, stream);
+}
+
+// codes, scales of silu(a g^T) * (a u^T), out_kp columns; w: strips of 32 rows of g and their 32 of u, 2 out_kp rows
+extern "C" int ti_mx_gemm_glu(const void* a, const void* a_scales, int a_bits, const void* w, const void* w_scales, void* codes,
+                              void* scales, int out_bits, int m, int out_kp, int kp, int settled, int* status, void* stream) {
+    if (int rc = check("mx_gemm_glu", a, a_scales, a_bits, w, w_scales, m, 2 * out_kp, kp)) return rc;
+    TI_REQUIRE(out_bits == 4 || out_bits == 8, "mx_gemm_glu: output of %d bits (4 and 8 are known)", out_bits);
+    TI_REQUIRE(out_kp % CHUNK == 0, "mx_gemm_glu: %d output columns are not whole chunks of 128", out_kp);
+    if (m == 0 || out_kp == 0) return 0;
+    const Args p{(const unsigned char*)w_scales, (const unsigned char*)a_scales, nullptr, (unsigned char*)codes,
+                 (unsigned char*)scales, m, 2 * out_kp, kp, 0, out_kp, MODE_GLU, 1, 0, settled, status};
+    if (out_bits == 8) return a_bits == 4 ? launch_rows<4, 8>(w, a, p, stream) : launch_rows<8, 8>(w, a, p, stream);
+    return a_bits == 4 ? launch_rows<4, 4>(w, a, p, stream) : launch_rows<8, 4>(w, a, p, stream);
+}

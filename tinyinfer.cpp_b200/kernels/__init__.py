@@ -1,6 +1,7 @@
 """Bindings of the hand-written CUDA kernels (sm_100a)."""
 from .build import BuildError, build_all, build_library, load_library, register_library
 from .cuda_ops import CudaOps, KernelError
+from .mx_ops import MxRows
 
 _OPS: dict[str, CudaOps] = {}
 
@@ -15,5 +16,5 @@ def cuda_ops(device) -> CudaOps:
     return _OPS[key]
 
 
-__all__ = ["BuildError", "CudaOps", "KernelError", "build_all", "build_library", "cuda_ops",
+__all__ = ["BuildError", "CudaOps", "KernelError", "MxRows", "build_all", "build_library", "cuda_ops",
            "load_library", "register_library"]

@@ -38,6 +38,8 @@ LIBRARIES = {
     "channels": ["common.cu", "channel_recurrence.cu"],
     # short convolutions over time, norms in groups and without statistics, depth sums, gated activations
     "rows": ["common.cu", "state_rows.cu", "layer_norm.cu"],
+    # microscaled rows and weights: quantisation, the norm into them, their products
+    "mx": ["common.cu", "mx_rows.cu", "mx_gemm.cu"],
 }
 
 # libraries that parts bring themselves: name -> (absolute source paths, include folders)

@@ -42,6 +42,7 @@ import torch
 
 from .build import load_library
 from .mixer_ops import MixerOps
+from .mx_ops import MxOps
 from .state_ops import StateOps
 
 _CODE = {torch.float32: 0, torch.bfloat16: 1}
@@ -133,7 +134,7 @@ def choose_prompt_attention(n_tiles: int, num_heads: int, num_sms: int, *, reach
     return two, runs
 
 
-class CudaOps(MixerOps, StateOps):
+class CudaOps(MixerOps, StateOps, MxOps):
     name = "cuda"
 
     def __init__(self, device):

@@ -64,6 +64,23 @@ __device__ __forceinline__ float value_e2m1(unsigned c) {
     return c & 8 ? -v : v;
 }
 
+// ---- clusters ------------------------------------------------------------------------------------
+
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n" ::: "memory");
+    asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ unsigned map_to_rank(unsigned addr, unsigned rank) {
+    unsigned out;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
+    return out;
+}
+
 // ---- block-scaled products -----------------------------------------------------------------------
 
 // Descriptor of 32 rows of 16 bytes without a swizzle: groups of 8 rows are 128 bytes apart.
@@ -107,4 +124,26 @@ inline int make_map_codes(CUtensorMap* map, const void* base, int rows, int kp, 
     return 0;
 }
 
+// the scale tiles of `rows` rows of `kp` elements as words; boxes of `chunks` tiles of one row of tiles
+inline int make_map_scales(CUtensorMap* map, const void* base, int rows, int kp, int chunks, const char* who) {
+    sm100::EncodeTiled fn = sm100::encode_fn();
+    if (!fn) return ti_fail("%s: the driver lacks cuTensorMapEncodeTiled", who);
+    const cuuint64_t bytes = (cuuint64_t)kp / CHUNK * TILE_BYTES;
+    const cuuint64_t dims[2] = {bytes / 4, (cuuint64_t)((rows + TILE_ROWS - 1) / TILE_ROWS)};
+    const cuuint64_t strides[1] = {bytes};
+    const cuuint32_t box[2] = {(cuuint32_t)(chunks * TILE_BYTES / 4), 1};
+    const cuuint32_t elem[2] = {1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 2, const_cast<void*>(base), dims, strides, box, elem,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return ti_fail("%s: cuTensorMapEncodeTiled failed with %d", who, (int)r);
+    return 0;
+}
+
 }  // namespace mx
+
+// mx_gemm_pairs.cu, called by the entry points of mx_gemm.cu
+int mx_gemm_pairs(const void* a, const void* a_scales, int a_bits, const void* w, const void* w_scales, float* c, int m, int n,
+                  int kp, int ldc, int accumulate, int settled, int* status, void* stream);
+int mx_gemm_pairs_glu(const void* a, const void* a_scales, int a_bits, const void* w, const void* w_scales, void* codes,
+                      void* scales, int out_bits, int m, int out_kp, int kp, int settled, int* status, void* stream);

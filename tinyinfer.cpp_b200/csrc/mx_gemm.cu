@@ -54,20 +54,6 @@ struct Args {
     int* status;
 };
 
-__device__ __forceinline__ unsigned cluster_rank() {
-    unsigned r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.aligned;\n" ::: "memory");
-    asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ unsigned map_to_rank(unsigned addr, unsigned rank) {
-    unsigned out;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
-    return out;
-}
 __device__ __forceinline__ float load_cluster(unsigned addr) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -347,6 +333,8 @@ template <int ABITS, int OBITS> int launch_rows(const void* w, const void* x, co
          : launch<256, ABITS, OBITS>(w, x, p, stream);
 }
 
+bool use_pairs(int m, int n) { return m > 256; }
+
 int check(const char* who, const void* a, const void* a_scales, int a_bits, const void* w, const void* w_scales, int m, int n,
           int kp) {
     TI_REQUIRE(a_bits == 4 || a_bits == 8, "%s: rows of %d bits (4 and 8 are known)", who, a_bits);
@@ -364,6 +352,8 @@ extern "C" int ti_mx_gemm(const void* a, const void* a_scales, int a_bits, const
     if (int rc = check("mx_gemm", a, a_scales, a_bits, w, w_scales, m, n, kp)) return rc;
     TI_REQUIRE((uintptr_t)c % 4 == 0 && ldc >= n, "mx_gemm: rows of %d floats for %d columns", ldc, n);
     if (m == 0 || n == 0) return 0;
+    if (use_pairs(m, n))
+        return mx_gemm_pairs(a, a_scales, a_bits, w, w_scales, c, m, n, kp, ldc, accumulate, settled, status, stream);
     const Args p{(const unsigned char*)w_scales, (const unsigned char*)a_scales, c, nullptr, nullptr, m, n, kp, ldc, 0,
                  accumulate ? MODE_ACCUMULATE : MODE_STORE, 1, 0, settled, status};
     return a_bits == 4 ? launch_rows<4, 8>(w, a, p, stream) : launch_rows<8, 8>(w, a, p, stream);
@@ -376,6 +366,8 @@ extern "C" int ti_mx_gemm_glu(const void* a, const void* a_scales, int a_bits, c
     TI_REQUIRE(out_bits == 4 || out_bits == 8, "mx_gemm_glu: output of %d bits (4 and 8 are known)", out_bits);
     TI_REQUIRE(out_kp % CHUNK == 0, "mx_gemm_glu: %d output columns are not whole chunks of 128", out_kp);
     if (m == 0 || out_kp == 0) return 0;
+    if (use_pairs(m, 2 * out_kp))
+        return mx_gemm_pairs_glu(a, a_scales, a_bits, w, w_scales, codes, scales, out_bits, m, out_kp, kp, settled, status, stream);
     const Args p{(const unsigned char*)w_scales, (const unsigned char*)a_scales, nullptr, (unsigned char*)codes,
                  (unsigned char*)scales, m, 2 * out_kp, kp, 0, out_kp, MODE_GLU, 1, 0, settled, status};
     if (out_bits == 8) return a_bits == 4 ? launch_rows<4, 8>(w, a, p, stream) : launch_rows<8, 8>(w, a, p, stream);

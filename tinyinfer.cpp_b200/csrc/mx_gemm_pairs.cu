@@ -1,0 +1,329 @@
+// Products of many microscaled rows with 4-bit microscaled weights on pairs of SMs (tcgen05 cta_group::2, block-scaled).
+//
+// Two blocks of a cluster compute one 256 x 256 tile of C: rows of A are the instruction's M side (128 a block), rows of W its
+// N side (each block fetches 128 of them, both tensor cores read both).  A stage is 128 bytes of every operand row (256
+// elements where both sides have 4 bits, 128 where A has 8) and the scale tiles of those elements: the block's own for A, all
+// of W's 256 rows.  The leader's MMA thread copies a stage's scale tiles into tensor memory (each SM's own copy from its own
+// shared memory) and issues the products.
+//
+// Tensor memory holds one accumulator of 256 columns and the scales of every stage; there is no room for a second one.  So the
+// eight epilogue warps read a tile's sums into registers (128 a thread), hand the accumulator back, and store from registers
+// while the next tile's products run.
+//
+// Every wait is bounded; on a timeout the block records status 2 and both blocks leave through the cluster barrier.
+#include "mx.cuh"
+
+namespace {
+
+using namespace sm100;
+using namespace mx;
+
+constexpr int BM = 256, BN = 256, THREADS = 320;        // TMA warp, MMA warp, eight epilogue warps
+constexpr int ROW = 128;                                // bytes of an operand row in a stage
+enum { MODE_STORE = 0, MODE_ACCUMULATE = 1, MODE_GLU = 2 };
+enum { TI_ERR_TIMEOUT = 2 };
+
+template <int ABITS> struct Pair {
+    static constexpr int ELEMS = ABITS == 4 ? 256 : 128, CHUNKS = ELEMS / CHUNK;
+    static constexpr int STAGE_A = 128 * ROW, STAGE_B = 128 * ROW, SCALES = CHUNKS * TILE_BYTES;      // per block
+    static constexpr int STAGES = 6;
+    static constexpr int SMEM = STAGES * (STAGE_A + STAGE_B + 3 * SCALES) + 1024 + 256;
+    // what TMA counts for a stage, both blocks: spread codes count as they are packed
+    static constexpr unsigned STAGE_BYTES = 2 * (STAGE_A + STAGE_B / (ABITS == 8 ? 2 : 1) + 3 * SCALES);
+    static constexpr int SCALE_COLS = CHUNKS * 12;       // A's four columns, W's eight, per chunk
+    static_assert(BN + STAGES * SCALE_COLS <= 512, "tensor memory");
+    static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+struct Args {
+    float* c;
+    unsigned char *out_codes, *out_scales;
+    int m, n, kp, ldc, out_kp, mode, settled;
+    int* status;
+};
+
+// A TMA tile load of a block of a pair: the data goes to this block's shared memory, the bytes are counted by the barrier at
+// `bar` (the leader's).
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, unsigned bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(unsigned bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void commit_pair(void* bar) {
+    const unsigned short mask = 3;
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
+        ::"r"(smem_u32(bar)), "h"(mask) : "memory");
+}
+__device__ __forceinline__ void copy_scales_pair(unsigned tmem, const void* tile) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(scale_desc(tile)) : "memory");
+}
+template <int ABITS>
+__device__ __forceinline__ void umma_scaled_pair(unsigned tmem_d, unsigned long long da, unsigned long long db, unsigned idesc,
+                                                 unsigned sfa, unsigned sfb, unsigned accumulate) {
+    if (ABITS == 4)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+            ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+            ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+// 32 columns of this thread's lane; complete only behind loads_done() of the same registers
+__device__ __forceinline__ void load32(unsigned taddr, unsigned* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+template <int N> __device__ __forceinline__ void loads_done(unsigned (&r)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));       // no use of a register moves in front of the wait
+}
+
+// 32 gates and their 32 ups of one row as codes of one block
+template <int OBITS>
+__device__ __forceinline__ void finish_glu(const Args& p, const unsigned* gate, const unsigned* up, int row, int out_col) {
+    float h[32];
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        h[i] = silu_mul(__uint_as_float(gate[i]), __uint_as_float(up[i]));
+        top = max(top, __float_as_uint(h[i]) & 0x7fffffffu);
+    }
+    const unsigned s = scale_byte<OBITS>(top);
+    const float inv = scale_inverse(s);
+    unsigned char* at = p.out_codes + ((size_t)row * p.out_kp + out_col) / (8 / OBITS);
+    unsigned w[OBITS];
+#pragma unroll
+    for (int i = 0; i < OBITS; ++i) {
+        w[i] = 0;
+#pragma unroll
+        for (int j = 0; j < 32 / OBITS; j += 2) {
+            const float a = h[i * (32 / OBITS) + j] * inv, b = h[i * (32 / OBITS) + j + 1] * inv;
+            w[i] |= (OBITS == 8 ? codes_e4m3x2(a, b) : codes_e2m1x2(a, b)) << (OBITS * j);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < OBITS; i += 4)
+        *reinterpret_cast<uint4*>(at + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    p.out_scales[scale_at(row, out_col / BLOCK, p.out_kp / CHUNK)] = (unsigned char)s;
+}
+
+template <int ABITS, int OBITS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                     const __grid_constant__ CUtensorMap map_as, const __grid_constant__ CUtensorMap map_ws, const Args p) {
+    using T = Pair<ABITS>;
+    constexpr int STAGES = T::STAGES, CHUNKS = T::CHUNKS;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char *stage_a = smem, *stage_b = smem + STAGES * T::STAGE_A, *stage_s = stage_b + STAGES * T::STAGE_B;
+    unsigned long long* bars = (unsigned long long*)(stage_s + STAGES * 3 * T::SCALES);
+    unsigned long long* full = bars;                     // [STAGES] used in the leader only
+    unsigned long long* empty = bars + STAGES;           // [STAGES] in both blocks
+    unsigned long long *acc_full = bars + 2 * STAGES, *acc_empty = bars + 2 * STAGES + 1;    // in both; in the leader only
+    unsigned* tmem_slot = (unsigned*)(bars + 2 * STAGES + 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned rank = cluster_rank();
+    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+    const int chunks = p.kp / CHUNK, num_kb = (chunks + CHUNKS - 1) / CHUNKS;
+    const int tiles_m = (p.m + BM - 1) / BM, num_tiles = tiles_m * ((p.n + BN - 1) / BN);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        mbar_init(acc_full, 1);
+        mbar_init(acc_empty, 16);
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n"
+                     ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    }
+    pdl_launch();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                                      // both blocks' barriers exist before any use
+    tc_fence_after();
+    const unsigned tmem_base = *tmem_slot;
+
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            auto load_w = [&](int tile, int kb, int s) {
+                const int n0 = tile / tiles_m * BN;
+                const unsigned bar = map_to_rank(smem_u32(&full[s]), 0);
+                if (rank == 0) mbar_expect_tx(&full[s], T::STAGE_BYTES);
+                tma_load_pair(stage_b + s * T::STAGE_B, &map_w, bar, kb * ROW, n0 + (int)rank * 128);
+                unsigned char* at = stage_s + s * 3 * T::SCALES + T::SCALES;
+                tma_load_pair(at, &map_ws, bar, kb * (T::SCALES / 4), n0 / TILE_ROWS);
+                tma_load_pair(at + T::SCALES, &map_ws, bar, kb * (T::SCALES / 4), n0 / TILE_ROWS + 1);
+            };
+            int primed = 0;
+            if (p.settled)                               // W is older than the kernel in front of this one
+                for (int tile = pair; tile < num_tiles && primed < STAGES; tile += num_pairs)
+                    for (int kb = 0; kb < num_kb && primed < STAGES; ++kb, ++primed) load_w(tile, kb, primed);
+            pdl_wait();
+            int it = 0;
+            for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+                const int m0 = tile % tiles_m * BM + (int)rank * 128;
+                for (int kb = 0; kb < num_kb; ++kb, ++it) {
+                    const int s = it % STAGES;
+                    if (it >= primed) {
+                        ok = mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1);
+                        if (!ok) break;
+                        load_w(tile, kb, s);
+                    }
+                    const unsigned bar = map_to_rank(smem_u32(&full[s]), 0);
+                    tma_load_pair(stage_a + s * T::STAGE_A, &map_a, bar, kb * ROW, m0);
+                    tma_load_pair(stage_s + s * 3 * T::SCALES, &map_as, bar, kb * (T::SCALES / 4), m0 / TILE_ROWS);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && lane == 0) {
+            const unsigned idesc = ABITS == 4 ? scaled_idesc(BM, BN, FOUR_E2M1, FOUR_E2M1)
+                                              : scaled_idesc(BM, BN, MIXED_E4M3, MIXED_E2M1);
+            int it = 0, local = 0;
+            for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local) {
+                ok = mbar_wait(acc_empty, (local & 1) ^ 1);
+                if (!ok) break;
+                tc_fence_after();
+                for (int kb = 0; kb < num_kb; ++kb, ++it) {
+                    const int s = it % STAGES, held = min(CHUNKS, chunks - kb * CHUNKS);
+                    ok = mbar_wait(&full[s], (it / STAGES) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const unsigned cols = tmem_base + BN + s * T::SCALE_COLS;
+                    const unsigned char* scales = stage_s + s * 3 * T::SCALES;
+                    for (int j = 0; j < held; ++j)
+#pragma unroll
+                        for (int t = 0; t < 3; ++t)
+                            copy_scales_pair(cols + j * 12 + t * 4, scales + t * T::SCALES + j * TILE_BYTES);
+                    const unsigned long long da = umma_desc(stage_a + s * T::STAGE_A), db = umma_desc(stage_b + s * T::STAGE_B);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const int j = ABITS == 4 ? kk / 2 : 0;
+                        if (j >= held) break;
+                        umma_scaled_pair<ABITS>(tmem_base, da + kk * 2, db + kk * 2, with_ids(idesc, ABITS == 4 ? kk % 2 * 2 : kk),
+                                                cols + j * 12, cols + j * 12 + 4, (kb | kk) != 0);
+                    }
+                    commit_pair(&empty[s]);
+                }
+                commit_pair(acc_full);
+            }
+        }
+    } else {
+        const int quarter = warp & 3, half = (warp - 2) >> 2;       // the lanes this warp may read; half of the columns
+        const bool by8 = (uintptr_t)p.c % 32 == 0 && p.ldc % 8 == 0 && p.n % 8 == 0;
+        const unsigned acc = tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)(half * 128);
+        pdl_wait();                                                 // the output belongs to the chain of launches
+        int local = 0;
+        for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local) {
+            const int row = tile % tiles_m * BM + (int)rank * 128 + quarter * 32 + lane;
+            const int n0 = tile / tiles_m * BN + half * 128;
+            ok = mbar_wait(acc_full, local & 1);
+            if (!ok) break;
+            tc_fence_after();
+            unsigned v[128];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load32(acc + 32 * i, v + 32 * i);
+            loads_done(v);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(acc_empty), 0));
+            if (row >= p.m) {
+            } else if (p.mode == MODE_GLU) {
+                finish_glu<OBITS>(p, v, v + 32, row, n0 / 2);
+                finish_glu<OBITS>(p, v + 64, v + 96, row, n0 / 2 + 32);
+            } else {
+                float* dst = p.c + (size_t)row * p.ldc + n0;
+                if (by8) {                                          // whole sectors: a thread's stores are a row each
+#pragma unroll
+                    for (int i = 0; i < 128; i += 8) {
+                        if (n0 + i < p.n) {
+                            float4 x = make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]),
+                                                   __uint_as_float(v[i + 3]));
+                            float4 y = make_float4(__uint_as_float(v[i + 4]), __uint_as_float(v[i + 5]),
+                                                   __uint_as_float(v[i + 6]), __uint_as_float(v[i + 7]));
+                            if (p.mode == MODE_ACCUMULATE) {
+                                const float4 a = __ldcg((const float4*)(dst + i)), b = __ldcg((const float4*)(dst + i + 4));
+                                x.x += a.x; x.y += a.y; x.z += a.z; x.w += a.w;
+                                y.x += b.x; y.y += b.y; y.z += b.z; y.w += b.w;
+                            }
+                            store_f32x8(dst + i, x, y);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i)
+                        if (n0 + i < p.n)
+                            dst[i] = (p.mode == MODE_ACCUMULATE ? __ldcg(dst + i) : 0.0f) + __uint_as_float(v[i]);
+                }
+            }
+            __syncwarp();
+        }
+    }
+    if (!ok) atomicCAS(p.status, 0, TI_ERR_TIMEOUT);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                                      // nobody leaves while its pair may still signal it
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(512u) : "memory");
+    }
+}
+
+template <int ABITS, int OBITS>
+int launch(const void* a, const void* a_scales, const void* w, const void* w_scales, const Args& p, void* stream) {
+    using T = Pair<ABITS>;
+    auto kernel = mx_gemm_pairs_kernel<ABITS, OBITS>;
+    CUtensorMap map_a, map_w, map_as, map_ws;
+    if (int rc = make_map_codes(&map_a, a, p.m, p.kp, ABITS, false, 128, "mx_gemm_pairs")) return rc;
+    if (int rc = make_map_codes(&map_w, w, p.n, p.kp, 4, ABITS == 8, 128, "mx_gemm_pairs")) return rc;
+    if (int rc = make_map_scales(&map_as, a_scales, p.m, p.kp, T::CHUNKS, "mx_gemm_pairs")) return rc;
+    if (int rc = make_map_scales(&map_ws, w_scales, p.n, p.kp, T::CHUNKS, "mx_gemm_pairs")) return rc;
+    static TiPerDevice configured;
+    if (configured.first_use()) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+        if (e != cudaSuccess) return ti_fail("mx_gemm_pairs: %s", cudaGetErrorString(e));
+        configured.mark();
+    }
+    int device = 0, sms = 0;
+    cudaGetDevice(&device);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    const int tiles = ((p.m + BM - 1) / BM) * ((p.n + BN - 1) / BN), pairs = tiles < sms / 2 ? tiles : sms / 2;
+    ti_launch_pdl(kernel, 2 * pairs, THREADS, T::SMEM, (cudaStream_t)stream, map_a, map_w, map_as, map_ws, p);
+    return ti_check_launch("mx_gemm_pairs");
+}
+
+}  // namespace
+
+// as ti_mx_gemm and ti_mx_gemm_glu (mx_gemm.cu), whose checks these run behind
+int mx_gemm_pairs(const void* a, const void* a_scales, int a_bits, const void* w, const void* w_scales, float* c, int m, int n,
+                  int kp, int ldc, int accumulate, int settled, int* status, void* stream) {
+    const Args p{c, nullptr, nullptr, m, n, kp, ldc, 0, accumulate ? MODE_ACCUMULATE : MODE_STORE, settled, status};
+    return a_bits == 4 ? launch<4, 8>(a, a_scales, w, w_scales, p, stream) : launch<8, 8>(a, a_scales, w, w_scales, p, stream);
+}
+int mx_gemm_pairs_glu(const void* a, const void* a_scales, int a_bits, const void* w, const void* w_scales, void* codes,
+                      void* scales, int out_bits, int m, int out_kp, int kp, int settled, int* status, void* stream) {
+    const Args p{nullptr, (unsigned char*)codes, (unsigned char*)scales, m, 2 * out_kp, kp, 0, out_kp, MODE_GLU, settled, status};
+    if (out_bits == 8)
+        return a_bits == 4 ? launch<4, 8>(a, a_scales, w, w_scales, p, stream) : launch<8, 8>(a, a_scales, w, w_scales, p, stream);
+    return a_bits == 4 ? launch<4, 4>(a, a_scales, w, w_scales, p, stream) : launch<8, 4>(a, a_scales, w, w_scales, p, stream);
+}

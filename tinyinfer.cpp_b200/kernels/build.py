@@ -39,7 +39,7 @@ LIBRARIES = {
     # short convolutions over time, norms in groups and without statistics, depth sums, gated activations
     "rows": ["common.cu", "state_rows.cu", "layer_norm.cu"],
     # microscaled rows and weights: quantisation, the norm into them, their products
-    "mx": ["common.cu", "mx_rows.cu", "mx_gemm.cu"],
+    "mx": ["common.cu", "mx_rows.cu", "mx_gemm.cu", "mx_gemm_pairs.cu"],
 }
 
 # libraries that parts bring themselves: name -> (absolute source paths, include folders)

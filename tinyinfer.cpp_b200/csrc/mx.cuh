@@ -9,8 +9,8 @@
 // In memory rows are padded with zeros to whole chunks of 128 elements (so that a row of operands for the tensor cores, 128
 // bytes of 4-bit codes unpacked or of 8-bit codes, never ends inside), two 4-bit codes share a byte, the even element low.
 // The scales of 128 rows and one chunk are 512 bytes, [row % 32][row / 32 % 4][block % 4], the tiles of a row's chunks one
-// behind the other: one tcgen05.cp of 32 rows of 128 bits brings such a tile into four columns of tensor memory, the form in
-// which the block-scaled products want it.  Rows up to the next multiple of 128 have scale bytes that nothing depends on.
+// behind the other: as 32 rows of 16 bytes such a tile is what the block-scaled products want in four columns of tensor
+// memory, once in each quarter of its lanes.  Rows up to the next multiple of 128 have scale bytes that nothing depends on.
 #pragma once
 
 #include "sm100.cuh"
@@ -83,11 +83,16 @@ __device__ __forceinline__ unsigned map_to_rank(unsigned addr, unsigned rank) {
 
 // ---- block-scaled products -----------------------------------------------------------------------
 
-// Descriptor of 32 rows of 16 bytes without a swizzle: groups of 8 rows are 128 bytes apart.
-__device__ __forceinline__ unsigned long long scale_desc(const void* p) {
-    return (unsigned long long)((sm100::smem_u32(p) & 0x3FFFF) >> 4) | (unsigned long long)1 << 16 |
-           (unsigned long long)(128 >> 4) << 32 | (unsigned long long)1 << 46;
+// A scale tile goes into tensor memory as its bytes lie: lane l of each quarter gets bytes 16 l to 16 l + 15 in four columns.
+// Threads store it (a tile is one 16-byte read of shared memory and one tcgen05.st per lane).  tcgen05.cp would do it without
+// threads, but runs in line with the products: 2.4 PFLOP/s of 4-bit products 0.17 us shorter per 256 of K without it, a
+// quarter of the time (4,096 x 6,144 x 4,096 65.1 -> 49.8 us, 2,048 x 24,576 x 4,096 115.8 -> 85.9 us).
+__device__ __forceinline__ void tmem_store4(unsigned taddr, const uint4& v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};\n"
+                 ::"r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+__device__ __forceinline__ void tmem_stores_done() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+
 // Instruction descriptor of a block-scaled product with power-of-two scales; the scale bytes of a step of K are chosen in
 // their 32-bit words by `id` (bits 4-5 for B, 29-30 for A).
 __device__ __forceinline__ unsigned scaled_idesc(int m, int n, unsigned a_type, unsigned b_type) {

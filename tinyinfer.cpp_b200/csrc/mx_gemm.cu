@@ -4,9 +4,9 @@
 // The roles of the operands are swapped: 128 rows of W are the instruction's M side, NTOK rows of A its N side, so a step of
 // few rows streams W once and wastes nothing on empty rows of A.  A stage of the ring is 128 bytes of every operand row: 256
 // elements where both sides have 4 bits, 128 where A has 8 (W's codes then take a byte each in shared memory; the spreading
-// is TMA's), with the scale tiles of those elements beside it.  The MMA thread copies a stage's scale tiles into tensor
-// memory columns of that stage (tcgen05.cp runs in order with the products behind it; columns are written again when the
-// stage's "empty" barrier has seen the products that read them).
+// is TMA's), with the scale tiles of those elements beside it.  The epilogue warps, idle until the sums are there, store a
+// stage's scale tiles into tensor memory columns of that stage (mx.cuh says why not tcgen05.cp); columns are written again
+// when the stage's "empty" barrier has seen the products that read them.
 //
 // K is cut over the blocks of a cluster: each keeps its part of the sum in its shared memory, and after a cluster barrier
 // every block adds the parts of its share of the tokens, in the order of the blocks (no atomics: the same bits each run).
@@ -65,9 +65,6 @@ __device__ __forceinline__ float4 load_cluster4(unsigned addr) {
                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ void copy_scales(unsigned tmem, const void* tile) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(scale_desc(tile)) : "memory");
-}
 template <int ABITS>
 __device__ __forceinline__ void umma_scaled(unsigned tmem_d, unsigned long long da, unsigned long long db, unsigned idesc,
                                             unsigned sfa, unsigned sfb, unsigned accumulate) {
@@ -111,8 +108,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     unsigned char* stage_x = smem + STAGES * T::STAGE_W;
     unsigned char* stage_s = smem + STAGES * (T::STAGE_W + T::STAGE_X);
     unsigned long long* bars = (unsigned long long*)(stage_s + STAGES * T::STAGE_S);
-    unsigned long long *full = bars, *empty = bars + STAGES, *acc_full = bars + 2 * STAGES;
-    unsigned* tmem_slot = (unsigned*)(bars + 2 * STAGES + 1);
+    unsigned long long *full = bars, *empty = bars + STAGES;             // operands: TMA -> MMA, MMA -> TMA
+    unsigned long long *scales_full = bars + 2 * STAGES, *scaled = bars + 3 * STAGES;     // scales: TMA -> epilogue warps -> MMA
+    unsigned long long* acc_full = bars + 4 * STAGES;
+    unsigned* tmem_slot = (unsigned*)(bars + 4 * STAGES + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int part = (int)cluster_rank(), unit = (int)blockIdx.x / p.parts;
@@ -121,7 +120,12 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     const int kb0 = (int)((long long)part * num_kb / p.parts), kb1 = (int)((long long)(part + 1) * num_kb / p.parts);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+            mbar_init(&scales_full[s], 1);
+            mbar_init(&scaled[s], 4);
+        }
         mbar_init(acc_full, 1);
         mbar_fence_init();
     }
@@ -136,16 +140,14 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     if (warp == 0) {
         if (lane == 0) {
             const int x_tiles = min(XTILES, (p.m - tok0 + TILE_ROWS - 1) / TILE_ROWS);
-            auto stage_bytes = [&](int held) {               // what TMA counts for a stage that holds `held` chunks: spread codes
-                                                             // count as they are packed, half of the space they take
-                return (unsigned)(T::STAGE_W / (ABITS == 8 ? 2 : 1) + T::STAGE_X + held * (1 + x_tiles) * TILE_BYTES);
-            };
             auto load_w = [&](int kb, int s) {
                 const int held = min(CHUNKS, chunks - kb * CHUNKS);
-                mbar_expect_tx(&full[s], stage_bytes(held));
+                // spread codes count as they are packed, half of the space they take
+                mbar_expect_tx(&full[s], T::STAGE_W / (ABITS == 8 ? 2 : 1) + T::STAGE_X);
+                mbar_expect_tx(&scales_full[s], (unsigned)(held * (1 + x_tiles) * TILE_BYTES));
                 tma_load_2d(stage_w + s * T::STAGE_W, &map_w, &full[s], kb * ROW, n0);
                 bulk_load(stage_s + s * T::STAGE_S, p.w_scales + ((size_t)(n0 / TILE_ROWS) * chunks + kb * CHUNKS) * TILE_BYTES,
-                          (unsigned)(held * TILE_BYTES), smem_u32(&full[s]));
+                          (unsigned)(held * TILE_BYTES), smem_u32(&scales_full[s]));
             };
             int primed = 0;
             if (p.settled)                                    // W is older than the kernel in front of this one
@@ -163,7 +165,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 for (int j = 0; j < x_tiles; ++j)
                     bulk_load(stage_s + s * T::STAGE_S + CHUNKS * (1 + j) * TILE_BYTES,
                               p.x_scales + ((size_t)(tok0 / TILE_ROWS + j) * chunks + kb * CHUNKS) * TILE_BYTES,
-                              (unsigned)(held * TILE_BYTES), smem_u32(&full[s]));
+                              (unsigned)(held * TILE_BYTES), smem_u32(&scales_full[s]));
             }
         }
     } else if (warp == 1) {
@@ -172,17 +174,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                                               : scaled_idesc(BW, NTOK, MIXED_E2M1, MIXED_E4M3);
             for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
                 const int s = it % STAGES, held = min(CHUNKS, chunks - kb * CHUNKS);
-                ok = mbar_wait(&full[s], (it / STAGES) & 1);
+                ok = mbar_wait(&full[s], (it / STAGES) & 1) && mbar_wait(&scaled[s], (it / STAGES) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 const unsigned cols = tmem_base + T::ACC_COLS + s * T::SCALE_COLS;
-                for (int j = 0; j < held; ++j) {              // columns of a chunk: W's four, then four per scale tile of A
-                    copy_scales(cols + j * 4 * (1 + XTILES), stage_s + s * T::STAGE_S + j * TILE_BYTES);
-#pragma unroll
-                    for (int t = 0; t < XTILES; ++t)
-                        copy_scales(cols + j * 4 * (1 + XTILES) + 4 * (1 + t),
-                                    stage_s + s * T::STAGE_S + (CHUNKS * (1 + t) + j) * TILE_BYTES);
-                }
                 const unsigned long long dw = umma_desc(stage_w + s * T::STAGE_W), dx = umma_desc(stage_x + s * T::STAGE_X);
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {              // 32 bytes of every row: 64 or 32 elements
@@ -198,10 +193,25 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         }
     } else {
         const int quarter = warp & 3, row = quarter * 32 + lane;
-        pdl_wait();                                           // C belongs to the chain of launches
-        ok = mbar_wait(acc_full, 0);
-        tc_fence_after();
         const unsigned acc = tmem_base + ((unsigned)(quarter * 32) << 16);
+        // a stage's scale tiles into the stage's columns: W's four, then four per tile of A, per chunk
+        for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+            const int s = it % STAGES, held = min(CHUNKS, chunks - kb * CHUNKS);
+            ok = mbar_wait(&scales_full[s], (it / STAGES) & 1);
+            if (!ok) break;
+            const uint4* from = reinterpret_cast<const uint4*>(stage_s + s * T::STAGE_S) + lane;
+            for (int j = 0; j < held; ++j)
+#pragma unroll
+                for (int t = 0; t <= XTILES; ++t)
+                    tmem_store4(acc + T::ACC_COLS + s * T::SCALE_COLS + (j * (1 + XTILES) + t) * 4, from[(t * CHUNKS + j) * 32]);
+            tmem_stores_done();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&scaled[s]);
+        }
+        pdl_wait();                                           // C belongs to the chain of launches
+        ok = ok && mbar_wait(acc_full, 0);
+        tc_fence_after();
         const int held_tok = min(NTOK, p.m - tok0);
         if (p.mode != MODE_GLU && p.parts == 1) {             // straight to C: a warp's lanes are 32 neighbouring columns
 #pragma unroll 1

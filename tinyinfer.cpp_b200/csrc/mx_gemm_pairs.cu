@@ -3,8 +3,8 @@
 // Two blocks of a cluster compute one 256 x 256 tile of C: rows of A are the instruction's M side (128 a block), rows of W its
 // N side (each block fetches 128 of them, both tensor cores read both).  A stage is 128 bytes of every operand row (256
 // elements where both sides have 4 bits, 128 where A has 8) and the scale tiles of those elements: the block's own for A, all
-// of W's 256 rows.  The leader's MMA thread copies a stage's scale tiles into tensor memory (each SM's own copy from its own
-// shared memory) and issues the products.
+// of W's 256 rows.  Four warps of each block store a stage's scale tiles into its tensor memory, the leader's MMA thread issues
+// the products.
 //
 // Tensor memory holds one accumulator of 256 columns and the scales of every stage; there is no room for a second one.  So the
 // eight epilogue warps read a tile's sums into registers (128 a thread), hand the accumulator back, and store from registers
@@ -18,7 +18,7 @@ namespace {
 using namespace sm100;
 using namespace mx;
 
-constexpr int BM = 256, BN = 256, THREADS = 320;        // TMA warp, MMA warp, eight epilogue warps
+constexpr int BM = 256, BN = 256, THREADS = 512;        // warpgroups: TMA and MMA warps, scale warps, two of epilogue
 constexpr int ROW = 128;                                // bytes of an operand row in a stage
 enum { MODE_STORE = 0, MODE_ACCUMULATE = 1, MODE_GLU = 2 };
 enum { TI_ERR_TIMEOUT = 2 };
@@ -27,9 +27,9 @@ template <int ABITS> struct Pair {
     static constexpr int ELEMS = ABITS == 4 ? 256 : 128, CHUNKS = ELEMS / CHUNK;
     static constexpr int STAGE_A = 128 * ROW, STAGE_B = 128 * ROW, SCALES = CHUNKS * TILE_BYTES;      // per block
     static constexpr int STAGES = 6;
-    static constexpr int SMEM = STAGES * (STAGE_A + STAGE_B + 3 * SCALES) + 1024 + 256;
+    static constexpr int SMEM = STAGES * (STAGE_A + STAGE_B + 3 * SCALES) + 1024 + 512;
     // what TMA counts for a stage, both blocks: spread codes count as they are packed
-    static constexpr unsigned STAGE_BYTES = 2 * (STAGE_A + STAGE_B / (ABITS == 8 ? 2 : 1) + 3 * SCALES);
+    static constexpr unsigned STAGE_BYTES = 2 * (STAGE_A + STAGE_B / (ABITS == 8 ? 2 : 1));
     static constexpr int SCALE_COLS = CHUNKS * 12;       // A's four columns, W's eight, per chunk
     static_assert(BN + STAGES * SCALE_COLS <= 512, "tensor memory");
     static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -57,9 +57,6 @@ __device__ __forceinline__ void commit_pair(void* bar) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
         ::"r"(smem_u32(bar)), "h"(mask) : "memory");
-}
-__device__ __forceinline__ void copy_scales_pair(unsigned tmem, const void* tile) {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(scale_desc(tile)) : "memory");
 }
 template <int ABITS>
 __device__ __forceinline__ void umma_scaled_pair(unsigned tmem_d, unsigned long long da, unsigned long long db, unsigned idesc,
@@ -135,8 +132,10 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     unsigned long long* bars = (unsigned long long*)(stage_s + STAGES * 3 * T::SCALES);
     unsigned long long* full = bars;                     // [STAGES] used in the leader only
     unsigned long long* empty = bars + STAGES;           // [STAGES] in both blocks
-    unsigned long long *acc_full = bars + 2 * STAGES, *acc_empty = bars + 2 * STAGES + 1;    // in both; in the leader only
-    unsigned* tmem_slot = (unsigned*)(bars + 2 * STAGES + 2);
+    unsigned long long* scales_full = bars + 2 * STAGES;  // [STAGES] in both blocks, each its own scales' bytes
+    unsigned long long* scaled = bars + 3 * STAGES;      // [STAGES] used in the leader only: scales are in tensor memory
+    unsigned long long *acc_full = bars + 4 * STAGES, *acc_empty = bars + 4 * STAGES + 1;    // in both; in the leader only
+    unsigned* tmem_slot = (unsigned*)(bars + 4 * STAGES + 2);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned rank = cluster_rank();
@@ -145,7 +144,12 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const int tiles_m = (p.m + BM - 1) / BM, num_tiles = tiles_m * ((p.n + BN - 1) / BN);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+            mbar_init(&scales_full[s], 1);
+            mbar_init(&scaled[s], 8);
+        }
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 16);
         mbar_fence_init();
@@ -163,73 +167,93 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const unsigned tmem_base = *tmem_slot;
 
     bool ok = true;
-    if (warp == 0) {
-        if (lane == 0) {
-            auto load_w = [&](int tile, int kb, int s) {
-                const int n0 = tile / tiles_m * BN;
-                const unsigned bar = map_to_rank(smem_u32(&full[s]), 0);
-                if (rank == 0) mbar_expect_tx(&full[s], T::STAGE_BYTES);
-                tma_load_pair(stage_b + s * T::STAGE_B, &map_w, bar, kb * ROW, n0 + (int)rank * 128);
-                unsigned char* at = stage_s + s * 3 * T::SCALES + T::SCALES;
-                tma_load_pair(at, &map_ws, bar, kb * (T::SCALES / 4), n0 / TILE_ROWS);
-                tma_load_pair(at + T::SCALES, &map_ws, bar, kb * (T::SCALES / 4), n0 / TILE_ROWS + 1);
-            };
-            int primed = 0;
-            if (p.settled)                               // W is older than the kernel in front of this one
-                for (int tile = pair; tile < num_tiles && primed < STAGES; tile += num_pairs)
-                    for (int kb = 0; kb < num_kb && primed < STAGES; ++kb, ++primed) load_w(tile, kb, primed);
-            pdl_wait();
-            int it = 0;
-            for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
-                const int m0 = tile % tiles_m * BM + (int)rank * 128;
-                for (int kb = 0; kb < num_kb; ++kb, ++it) {
-                    const int s = it % STAGES;
-                    if (it >= primed) {
-                        ok = mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1);
-                        if (!ok) break;
-                        load_w(tile, kb, s);
-                    }
+    // Registers: the block starts with 128 a thread; an epilogue thread needs its 128 sums and what it stores them with (160
+    // bytes of spills without the exchange: 53.0 -> 49.8 us at 4,096 x 6,144 x 4,096).  2 x 88 + 2 x 168 = 4 x 128.
+    if (warp < 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
+        if (warp == 0) {
+            if (lane == 0) {
+                auto load_w = [&](int tile, int kb, int s) {
+                    const int n0 = tile / tiles_m * BN;
                     const unsigned bar = map_to_rank(smem_u32(&full[s]), 0);
-                    tma_load_pair(stage_a + s * T::STAGE_A, &map_a, bar, kb * ROW, m0);
-                    tma_load_pair(stage_s + s * 3 * T::SCALES, &map_as, bar, kb * (T::SCALES / 4), m0 / TILE_ROWS);
+                    if (rank == 0) mbar_expect_tx(&full[s], T::STAGE_BYTES);
+                    mbar_expect_tx(&scales_full[s], 3 * T::SCALES);
+                    tma_load_pair(stage_b + s * T::STAGE_B, &map_w, bar, kb * ROW, n0 + (int)rank * 128);
+                    unsigned char* at = stage_s + s * 3 * T::SCALES + T::SCALES;
+                    tma_load_2d(at, &map_ws, &scales_full[s], kb * (T::SCALES / 4), n0 / TILE_ROWS);
+                    tma_load_2d(at + T::SCALES, &map_ws, &scales_full[s], kb * (T::SCALES / 4), n0 / TILE_ROWS + 1);
+                };
+                int primed = 0;
+                if (p.settled)                               // W is older than the kernel in front of this one
+                    for (int tile = pair; tile < num_tiles && primed < STAGES; tile += num_pairs)
+                        for (int kb = 0; kb < num_kb && primed < STAGES; ++kb, ++primed) load_w(tile, kb, primed);
+                pdl_wait();
+                int it = 0;
+                for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+                    const int m0 = tile % tiles_m * BM + (int)rank * 128;
+                    for (int kb = 0; kb < num_kb; ++kb, ++it) {
+                        const int s = it % STAGES;
+                        if (it >= primed) {
+                            ok = mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1);
+                            if (!ok) break;
+                            load_w(tile, kb, s);
+                        }
+                        const unsigned bar = map_to_rank(smem_u32(&full[s]), 0);
+                        tma_load_pair(stage_a + s * T::STAGE_A, &map_a, bar, kb * ROW, m0);
+                        tma_load_2d(stage_s + s * 3 * T::SCALES, &map_as, &scales_full[s], kb * (T::SCALES / 4), m0 / TILE_ROWS);
+                    }
                 }
             }
-        }
-    } else if (warp == 1) {
-        if (rank == 0 && lane == 0) {
-            const unsigned idesc = ABITS == 4 ? scaled_idesc(BM, BN, FOUR_E2M1, FOUR_E2M1)
-                                              : scaled_idesc(BM, BN, MIXED_E4M3, MIXED_E2M1);
-            int it = 0, local = 0;
-            for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local) {
-                ok = mbar_wait(acc_empty, (local & 1) ^ 1);
-                if (!ok) break;
-                tc_fence_after();
-                for (int kb = 0; kb < num_kb; ++kb, ++it) {
-                    const int s = it % STAGES, held = min(CHUNKS, chunks - kb * CHUNKS);
-                    ok = mbar_wait(&full[s], (it / STAGES) & 1);
+        } else if (warp == 1) {
+            if (rank == 0 && lane == 0) {
+                const unsigned idesc = ABITS == 4 ? scaled_idesc(BM, BN, FOUR_E2M1, FOUR_E2M1)
+                                                  : scaled_idesc(BM, BN, MIXED_E4M3, MIXED_E2M1);
+                int it = 0, local = 0;
+                for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local) {
+                    ok = mbar_wait(acc_empty, (local & 1) ^ 1);
                     if (!ok) break;
                     tc_fence_after();
-                    const unsigned cols = tmem_base + BN + s * T::SCALE_COLS;
-                    const unsigned char* scales = stage_s + s * 3 * T::SCALES;
-                    for (int j = 0; j < held; ++j)
+                    for (int kb = 0; kb < num_kb; ++kb, ++it) {
+                        const int s = it % STAGES, held = min(CHUNKS, chunks - kb * CHUNKS);
+                        ok = mbar_wait(&full[s], (it / STAGES) & 1) && mbar_wait(&scaled[s], (it / STAGES) & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const unsigned cols = tmem_base + BN + s * T::SCALE_COLS;
+                        const unsigned long long da = umma_desc(stage_a + s * T::STAGE_A), db = umma_desc(stage_b + s * T::STAGE_B);
 #pragma unroll
-                        for (int t = 0; t < 3; ++t)
-                            copy_scales_pair(cols + j * 12 + t * 4, scales + t * T::SCALES + j * TILE_BYTES);
-                    const unsigned long long da = umma_desc(stage_a + s * T::STAGE_A), db = umma_desc(stage_b + s * T::STAGE_B);
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        const int j = ABITS == 4 ? kk / 2 : 0;
-                        if (j >= held) break;
-                        umma_scaled_pair<ABITS>(tmem_base, da + kk * 2, db + kk * 2, with_ids(idesc, ABITS == 4 ? kk % 2 * 2 : kk),
-                                                cols + j * 12, cols + j * 12 + 4, (kb | kk) != 0);
+                        for (int kk = 0; kk < 4; ++kk) {
+                            const int j = ABITS == 4 ? kk / 2 : 0;
+                            if (j >= held) break;
+                            umma_scaled_pair<ABITS>(tmem_base, da + kk * 2, db + kk * 2, with_ids(idesc, ABITS == 4 ? kk % 2 * 2 : kk),
+                                                    cols + j * 12, cols + j * 12 + 4, (kb | kk) != 0);
+                        }
+                        commit_pair(&empty[s]);
                     }
-                    commit_pair(&empty[s]);
+                    commit_pair(acc_full);
                 }
-                commit_pair(acc_full);
+            }
+        } else if (warp >= 4) {
+            // A stage's scale tiles into the stage's columns of tensor memory, each warp its 32 lanes.
+            const unsigned acc = tmem_base + ((unsigned)((warp & 3) * 32) << 16) + BN;
+            const int mine = num_tiles > pair ? (num_tiles - pair + num_pairs - 1) / num_pairs : 0;
+            for (int it = 0; it < mine * num_kb; ++it) {
+                const int s = it % STAGES;
+                ok = mbar_wait(&scales_full[s], (it / STAGES) & 1);
+                if (!ok) break;
+                const uint4* from = reinterpret_cast<const uint4*>(stage_s + s * 3 * T::SCALES) + lane;
+#pragma unroll
+                for (int j = 0; j < CHUNKS; ++j)
+#pragma unroll
+                    for (int t = 0; t < 3; ++t) tmem_store4(acc + s * T::SCALE_COLS + j * 12 + t * 4, from[(t * CHUNKS + j) * 32]);
+                tmem_stores_done();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&scaled[s]), 0));
             }
         }
     } else {
-        const int quarter = warp & 3, half = (warp - 2) >> 2;       // the lanes this warp may read; half of the columns
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n");
+        const int quarter = warp & 3, half = (warp - 8) >> 2;       // the lanes this warp may read; half of the columns
         const bool by8 = (uintptr_t)p.c % 32 == 0 && p.ldc % 8 == 0 && p.n % 8 == 0;
         const unsigned acc = tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)(half * 128);
         pdl_wait();                                                 // the output belongs to the chain of launches

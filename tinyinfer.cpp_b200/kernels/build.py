@@ -39,8 +39,10 @@ LIBRARIES = {
     # short convolutions over time, norms in groups and without statistics, depth sums, gated activations
     "rows": ["common.cu", "state_rows.cu", "layer_norm.cu"],
     # microscaled rows and weights: quantisation, the norm into them, their products
-    "mx": ["common.cu", "mx_rows.cu", "mx_gemm.cu", "mx_gemm_pairs.cu"],
+    "mx": ["common.cu", "mx_rows.cu", "mx_gemm.cu", "mx_gemm_pairs.cu", "mx_binding.cpp"],
 }
+# libraries that are Python modules too: they take torch's tensors as they are and link its libraries
+TORCH_MODULES = {"mx": "ti_mx"}
 
 # libraries that parts bring themselves: name -> (absolute source paths, include folders)
 _EXTRA: dict[str, tuple[list[str], list[str]]] = {}
@@ -110,9 +112,24 @@ def build_dir() -> str:
     raise BuildError("no writable folder for the compiled kernels: tried " + ", ".join(cands))
 
 
-def _digest(sources: list[str], include_dirs: list[str]) -> str:
+def _torch_flags() -> tuple[list[str], list[str]]:
+    """Compiler and linker flags of a library that is a Python module over torch's tensors.  torch is loaded before it, so
+    its libraries are found by name."""
+    import sysconfig
+
+    import torch
+    home = os.path.dirname(torch.__file__)
+    # the host compiler hides what these headers warn of behind -isystem
+    return (["-isystem", os.path.join(home, "include"), "-isystem", sysconfig.get_paths()["include"]],
+            ["-L", os.path.join(home, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"])
+
+
+def _digest(sources: list[str], include_dirs: list[str], module: bool = False) -> str:
     h = hashlib.sha256()
     h.update(" ".join(NVCC_FLAGS).encode())
+    if module:                                         # built against one torch and one Python
+        import torch
+        h.update(f"{torch.__version__} {sys.version}".encode())
     headers = []
     for d in [CSRC, *include_dirs]:
         headers += sorted(os.path.join(d, n) for n in os.listdir(d) if n.endswith((".cuh", ".h")))
@@ -158,7 +175,8 @@ def build_library(name: str, verbose: bool = True) -> str:
     out_dir = build_dir()
     so_path = os.path.join(out_dir, f"libtinyinfer_b200_{name}.so")
     stamp = so_path + ".sha256"
-    digest = _digest(sources, include_dirs)
+    module = name in TORCH_MODULES
+    digest = _digest(sources, include_dirs, module)
     with open(os.path.join(out_dir, f".{name}.lock"), "w") as lock:
         fcntl.flock(lock, fcntl.LOCK_EX)
         try:
@@ -176,14 +194,16 @@ def build_library(name: str, verbose: bool = True) -> str:
             includes = [x for d in [CSRC, *include_dirs] for x in ("-I", d)]
             if name not in LIBRARIES:                  # ti_fail and friends live in common.cu
                 sources = [os.path.join(CSRC, "common.cu"), *sources]
+            torch_flags, links = _torch_flags() if module else ([], [])
             for path in sources:
                 src = os.path.basename(path)
                 obj = os.path.join(out_dir, f"{name}_{os.path.splitext(src)[0]}.o")
                 objs[src] = obj
-                cmds[src] = [nvcc, *NVCC_FLAGS, *includes, "-c", path, "-o", obj]
+                extra = torch_flags if src.endswith(".cpp") else []
+                cmds[src] = [nvcc, *NVCC_FLAGS, *includes, *extra, "-c", path, "-o", obj]
             _run_all(cmds, f"'{name}' kernels")
             tmp = so_path + f".tmp{os.getpid()}"
-            _run_all({"link": [nvcc, "-shared", "-o", tmp, *objs.values()]},
+            _run_all({"link": [nvcc, "-shared", "-o", tmp, *objs.values(), *links]},
                      f"'{name}' kernels")
             os.replace(tmp, so_path)
             with open(stamp, "w") as fh:
@@ -196,12 +216,24 @@ def build_library(name: str, verbose: bool = True) -> str:
 
 
 _LOADED: dict[str, ctypes.CDLL] = {}
+_MODULES: dict = {}
 
 
 def load_library(name: str) -> ctypes.CDLL:
     if name not in _LOADED:
         _LOADED[name] = ctypes.CDLL(build_library(name))
     return _LOADED[name]
+
+
+def load_module(name: str):
+    """A library of ``TORCH_MODULES`` as the Python module it is."""
+    if name not in _MODULES:
+        import importlib.util
+        spec = importlib.util.spec_from_file_location(TORCH_MODULES[name], build_library(name))
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _MODULES[name] = module
+    return _MODULES[name]
 
 
 def build_all(verbose: bool = True) -> list[str]:

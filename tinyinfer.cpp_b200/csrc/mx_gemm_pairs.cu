@@ -1,10 +1,14 @@
 // Products of many microscaled rows with 4-bit microscaled weights on pairs of SMs (tcgen05 cta_group::2, block-scaled).
 //
-// Two blocks of a cluster compute one 256 x 256 tile of C: rows of A are the instruction's M side (128 a block), rows of W its
-// N side (each block fetches 128 of them, both tensor cores read both).  A stage is 128 bytes of every operand row (256
-// elements where both sides have 4 bits, 128 where A has 8) and the scale tiles of those elements: the block's own for A, all
-// of W's 256 rows.  Four warps of each block store a stage's scale tiles into its tensor memory, the leader's MMA thread issues
-// the products.
+// Two blocks of a cluster compute one tile of 256 rows of A and 256 rows of W together; each fetches 128 rows of either, both
+// tensor cores read both blocks' N side.  A stage is 128 bytes of every operand row (256 elements where both sides have 4
+// bits, 128 where A has 8) and the scale tiles of those elements: the block's own rows' for the M side, all 256 rows' for the
+// N side.  Four warps of each block store a stage's scale tiles into its tensor memory, the leader's MMA thread issues the
+// products.
+//
+// The gated form has A's rows on the M side: a thread then holds a row's 32 gates and their 32 ups, a block of the format.
+// The plain form has W's rows there: a warp's lanes are 32 neighbouring columns of C, whose stores and, when adding to C, loads
+// are whole lines (a row of C per lane instead, in stores of 32 bytes: XXX).
 //
 // Tensor memory holds one accumulator of 256 columns and the scales of every stage; there is no room for a second one.  So the
 // eight epilogue warps read a tile's sums into registers (128 a thread), hand the accumulator back, and store from registers
@@ -20,17 +24,16 @@ using namespace mx;
 
 constexpr int BM = 256, BN = 256, THREADS = 512;        // warpgroups: TMA and MMA warps, scale warps, two of epilogue
 constexpr int ROW = 128;                                // bytes of an operand row in a stage
-enum { MODE_STORE = 0, MODE_ACCUMULATE = 1, MODE_GLU = 2 };
 enum { TI_ERR_TIMEOUT = 2 };
 
 template <int ABITS> struct Pair {
     static constexpr int ELEMS = ABITS == 4 ? 256 : 128, CHUNKS = ELEMS / CHUNK;
-    static constexpr int STAGE_A = 128 * ROW, STAGE_B = 128 * ROW, SCALES = CHUNKS * TILE_BYTES;      // per block
+    static constexpr int SIDE = 128 * ROW, SCALES = CHUNKS * TILE_BYTES;      // operand rows and scale tiles of a block
     static constexpr int STAGES = 6;
-    static constexpr int SMEM = STAGES * (STAGE_A + STAGE_B + 3 * SCALES) + 1024 + 512;
+    static constexpr int SMEM = STAGES * (2 * SIDE + 3 * SCALES) + 1024 + 512;
     // what TMA counts for a stage, both blocks: spread codes count as they are packed
-    static constexpr unsigned STAGE_BYTES = 2 * (STAGE_A + STAGE_B / (ABITS == 8 ? 2 : 1));
-    static constexpr int SCALE_COLS = CHUNKS * 12;       // A's four columns, W's eight, per chunk
+    static constexpr unsigned STAGE_BYTES = 2 * (SIDE + SIDE / (ABITS == 8 ? 2 : 1));
+    static constexpr int SCALE_COLS = CHUNKS * 12;       // the M side's four columns, the N side's eight, per chunk
     static_assert(BN + STAGES * SCALE_COLS <= 512, "tensor memory");
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -38,7 +41,7 @@ template <int ABITS> struct Pair {
 struct Args {
     float* c;
     unsigned char *out_codes, *out_scales;
-    int m, n, kp, ldc, out_kp, mode, settled;
+    int m, n, kp, ldc, out_kp, accumulate, settled;
     int* status;
 };
 
@@ -120,15 +123,16 @@ __device__ __forceinline__ void finish_glu(const Args& p, const unsigned* gate, 
     p.out_scales[scale_at(row, out_col / BLOCK, p.out_kp / CHUNK)] = (unsigned char)s;
 }
 
-template <int ABITS, int OBITS>
+// map_p, map_ps: codes and scales of the M side, map_q, map_qs: of the N side.  GLU: the M side is A, the output codes.
+template <int ABITS, int OBITS, bool GLU>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
-                     const __grid_constant__ CUtensorMap map_as, const __grid_constant__ CUtensorMap map_ws, const Args p) {
+mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                     const __grid_constant__ CUtensorMap map_ps, const __grid_constant__ CUtensorMap map_qs, const Args p) {
     using T = Pair<ABITS>;
     constexpr int STAGES = T::STAGES, CHUNKS = T::CHUNKS;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    unsigned char *stage_a = smem, *stage_b = smem + STAGES * T::STAGE_A, *stage_s = stage_b + STAGES * T::STAGE_B;
+    unsigned char *stage_p = smem, *stage_q = smem + STAGES * T::SIDE, *stage_s = stage_q + STAGES * T::SIDE;
     unsigned long long* bars = (unsigned long long*)(stage_s + STAGES * 3 * T::SCALES);
     unsigned long long* full = bars;                     // [STAGES] used in the leader only
     unsigned long long* empty = bars + STAGES;           // [STAGES] in both blocks
@@ -141,7 +145,7 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const unsigned rank = cluster_rank();
     const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
     const int chunks = p.kp / CHUNK, num_kb = (chunks + CHUNKS - 1) / CHUNKS;
-    const int tiles_m = (p.m + BM - 1) / BM, num_tiles = tiles_m * ((p.n + BN - 1) / BN);
+    const int tiles_a = (p.m + 255) / 256, num_tiles = tiles_a * ((p.n + 255) / 256);     // neighbours share rows of W
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -168,58 +172,71 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
 
     bool ok = true;
     // Registers: the block starts with 128 a thread; an epilogue thread needs its 128 sums and what it stores them with (160
-    // bytes of spills without the exchange: 53.0 -> 49.8 us at 4,096 x 6,144 x 4,096).  2 x 88 + 2 x 168 = 4 x 128.
+    // bytes of spills without the exchange: 53.0 -> 49.8 us at 4,096 x 6,144 x 4,096).  2 x 72 + 2 x 184 = 4 x 128.
     if (warp < 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
         if (warp == 0) {
             if (lane == 0) {
-                auto load_w = [&](int tile, int kb, int s) {
-                    const int n0 = tile / tiles_m * BN;
-                    const unsigned bar = map_to_rank(smem_u32(&full[s]), 0);
+                    const unsigned full0 = map_to_rank(smem_u32(full), 0);    // the leader's barriers
+                auto expect = [&](int s) {
                     if (rank == 0) mbar_expect_tx(&full[s], T::STAGE_BYTES);
                     mbar_expect_tx(&scales_full[s], 3 * T::SCALES);
-                    tma_load_pair(stage_b + s * T::STAGE_B, &map_w, bar, kb * ROW, n0 + (int)rank * 128);
-                    unsigned char* at = stage_s + s * 3 * T::SCALES + T::SCALES;
-                    tma_load_2d(at, &map_ws, &scales_full[s], kb * (T::SCALES / 4), n0 / TILE_ROWS);
-                    tma_load_2d(at + T::SCALES, &map_ws, &scales_full[s], kb * (T::SCALES / 4), n0 / TILE_ROWS + 1);
+                };
+                auto load_p = [&](int row, int kb, int s) {       // the block's own rows
+                    tma_load_pair(stage_p + s * T::SIDE, &map_p, full0 + 8 * s, kb * ROW, row);
+                    tma_load_2d(stage_s + s * 3 * T::SCALES, &map_ps, &scales_full[s], kb * (T::SCALES / 4), row / TILE_ROWS);
+                };
+                auto load_q = [&](int row, int kb, int s) {       // half of the tile's rows, the scales of all
+                    tma_load_pair(stage_q + s * T::SIDE, &map_q, full0 + 8 * s, kb * ROW, row + (int)rank * 128);
+                    unsigned char* at = stage_s + (s * 3 + 1) * T::SCALES;
+                    for (int t = 0; t < 2; ++t)
+                        tma_load_2d(at + t * T::SCALES, &map_qs, &scales_full[s], kb * (T::SCALES / 4), row / TILE_ROWS + t);
                 };
                 int primed = 0;
-                if (p.settled)                               // W is older than the kernel in front of this one
-                    for (int tile = pair; tile < num_tiles && primed < STAGES; tile += num_pairs)
-                        for (int kb = 0; kb < num_kb && primed < STAGES; ++kb, ++primed) load_w(tile, kb, primed);
-                pdl_wait();
-                int it = 0;
-                for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
-                    const int m0 = tile % tiles_m * BM + (int)rank * 128;
-                    for (int kb = 0; kb < num_kb; ++kb, ++it) {
-                        const int s = it % STAGES;
-                        if (it >= primed) {
-                            ok = mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1);
-                            if (!ok) break;
-                            load_w(tile, kb, s);
+                if (p.settled)                           // W is older than the kernel in front of this one
+                    for (int tile = pair; tile < num_tiles && primed < STAGES; tile += num_pairs) {
+                        const int w0 = tile / tiles_a * 256;
+                        for (int kb = 0; kb < num_kb && primed < STAGES; ++kb, ++primed) {
+                            expect(primed);
+                            if (GLU) load_q(w0, kb, primed);
+                            else load_p(w0 + (int)rank * 128, kb, primed);
                         }
-                        const unsigned bar = map_to_rank(smem_u32(&full[s]), 0);
-                        tma_load_pair(stage_a + s * T::STAGE_A, &map_a, bar, kb * ROW, m0);
-                        tma_load_2d(stage_s + s * 3 * T::SCALES, &map_as, &scales_full[s], kb * (T::SCALES / 4), m0 / TILE_ROWS);
+                    }
+                pdl_wait();
+                int s = 0, it = 0;
+                unsigned phase = 1;                      // of "empty"
+                for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+                    const int a0 = tile % tiles_a * 256, w0 = tile / tiles_a * 256;
+                    const int p0 = (GLU ? a0 : w0) + (int)rank * 128, q0 = GLU ? w0 : a0;
+                    for (int kb = 0; kb < num_kb; ++kb, ++it) {
+                        if (it >= primed) {
+                            ok = mbar_wait(&empty[s], phase);
+                            if (!ok) break;
+                            expect(s);
+                        }
+                        if (!GLU || it >= primed) load_q(q0, kb, s);
+                        if (GLU || it >= primed) load_p(p0, kb, s);
+                        if (++s == STAGES) s = 0, phase ^= 1;
                     }
                 }
             }
         } else if (warp == 1) {
             if (rank == 0 && lane == 0) {
                 const unsigned idesc = ABITS == 4 ? scaled_idesc(BM, BN, FOUR_E2M1, FOUR_E2M1)
-                                                  : scaled_idesc(BM, BN, MIXED_E4M3, MIXED_E2M1);
-                int it = 0, local = 0;
+                                     : GLU ? scaled_idesc(BM, BN, MIXED_E4M3, MIXED_E2M1) : scaled_idesc(BM, BN, MIXED_E2M1, MIXED_E4M3);
+                int s = 0, local = 0;
+                unsigned phase = 0;
                 for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local) {
                     ok = mbar_wait(acc_empty, (local & 1) ^ 1);
                     if (!ok) break;
                     tc_fence_after();
-                    for (int kb = 0; kb < num_kb; ++kb, ++it) {
-                        const int s = it % STAGES, held = min(CHUNKS, chunks - kb * CHUNKS);
-                        ok = mbar_wait(&full[s], (it / STAGES) & 1) && mbar_wait(&scaled[s], (it / STAGES) & 1);
+                    for (int kb = 0; kb < num_kb; ++kb) {
+                        const int held = min(CHUNKS, chunks - kb * CHUNKS);
+                        ok = mbar_wait(&full[s], phase) && mbar_wait(&scaled[s], phase);
                         if (!ok) break;
                         tc_fence_after();
                         const unsigned cols = tmem_base + BN + s * T::SCALE_COLS;
-                        const unsigned long long da = umma_desc(stage_a + s * T::STAGE_A), db = umma_desc(stage_b + s * T::STAGE_B);
+                        const unsigned long long da = umma_desc(stage_p + s * T::SIDE), db = umma_desc(stage_q + s * T::SIDE);
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) {
                             const int j = ABITS == 4 ? kk / 2 : 0;
@@ -228,6 +245,7 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                                                     cols + j * 12, cols + j * 12 + 4, (kb | kk) != 0);
                         }
                         commit_pair(&empty[s]);
+                        if (++s == STAGES) s = 0, phase ^= 1;
                     }
                     commit_pair(acc_full);
                 }
@@ -252,15 +270,13 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;\n");
         const int quarter = warp & 3, half = (warp - 8) >> 2;       // the lanes this warp may read; half of the columns
-        const bool by8 = (uintptr_t)p.c % 32 == 0 && p.ldc % 8 == 0 && p.n % 8 == 0;
         const unsigned acc = tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)(half * 128);
         pdl_wait();                                                 // the output belongs to the chain of launches
         int local = 0;
         for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local) {
-            const int row = tile % tiles_m * BM + (int)rank * 128 + quarter * 32 + lane;
-            const int n0 = tile / tiles_m * BN + half * 128;
+            const int tok0 = tile % tiles_a * 256, n0 = tile / tiles_a * 256, mine = (int)rank * 128 + quarter * 32 + lane;
             ok = mbar_wait(acc_full, local & 1);
             if (!ok) break;
             tc_fence_after();
@@ -271,33 +287,29 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(acc_empty), 0));
-            if (row >= p.m) {
-            } else if (p.mode == MODE_GLU) {
-                finish_glu<OBITS>(p, v, v + 32, row, n0 / 2);
-                finish_glu<OBITS>(p, v + 64, v + 96, row, n0 / 2 + 32);
+            if (GLU) {
+                const int row = tok0 + mine, col = (n0 + half * 128) / 2;
+                if (row < p.m) {
+                    finish_glu<OBITS>(p, v, v + 32, row, col);
+                    finish_glu<OBITS>(p, v + 64, v + 96, row, col + 32);
+                }
             } else {
-                float* dst = p.c + (size_t)row * p.ldc + n0;
-                if (by8) {                                          // whole sectors: a thread's stores are a row each
+                const int tok = tok0 + half * 128, held = p.m - tok;
+                if (n0 + mine < p.n) {
+                    float* dst = p.c + (size_t)tok * p.ldc + n0 + mine;
 #pragma unroll
-                    for (int i = 0; i < 128; i += 8) {
-                        if (n0 + i < p.n) {
-                            float4 x = make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]),
-                                                   __uint_as_float(v[i + 3]));
-                            float4 y = make_float4(__uint_as_float(v[i + 4]), __uint_as_float(v[i + 5]),
-                                                   __uint_as_float(v[i + 6]), __uint_as_float(v[i + 7]));
-                            if (p.mode == MODE_ACCUMULATE) {
-                                const float4 a = __ldcg((const float4*)(dst + i)), b = __ldcg((const float4*)(dst + i + 4));
-                                x.x += a.x; x.y += a.y; x.z += a.z; x.w += a.w;
-                                y.x += b.x; y.y += b.y; y.z += b.z; y.w += b.w;
-                            }
-                            store_f32x8(dst + i, x, y);
+                    for (int t0 = 0; t0 < 128; t0 += 32) {
+                        if (p.accumulate) {                         // old values are asked for 32 at a time
+                            float old[32];
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) old[i] = t0 + i < held ? __ldcg(dst + (size_t)(t0 + i) * p.ldc) : 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[t0 + i] = __float_as_uint(old[i] + __uint_as_float(v[t0 + i]));
                         }
-                    }
-                } else {
 #pragma unroll
-                    for (int i = 0; i < 128; ++i)
-                        if (n0 + i < p.n)
-                            dst[i] = (p.mode == MODE_ACCUMULATE ? __ldcg(dst + i) : 0.0f) + __uint_as_float(v[i]);
+                        for (int i = 0; i < 32; ++i)
+                            if (t0 + i < held) dst[(size_t)(t0 + i) * p.ldc] = __uint_as_float(v[t0 + i]);
+                    }
                 }
             }
             __syncwarp();
@@ -313,10 +325,10 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     }
 }
 
-template <int ABITS, int OBITS>
+template <int ABITS, int OBITS, bool GLU>
 int launch(const void* a, const void* a_scales, const void* w, const void* w_scales, const Args& p, void* stream) {
     using T = Pair<ABITS>;
-    auto kernel = mx_gemm_pairs_kernel<ABITS, OBITS>;
+    auto kernel = mx_gemm_pairs_kernel<ABITS, OBITS, GLU>;
     CUtensorMap map_a, map_w, map_as, map_ws;
     if (int rc = make_map_codes(&map_a, a, p.m, p.kp, ABITS, false, 128, "mx_gemm_pairs")) return rc;
     if (int rc = make_map_codes(&map_w, w, p.n, p.kp, 4, ABITS == 8, 128, "mx_gemm_pairs")) return rc;
@@ -331,8 +343,9 @@ int launch(const void* a, const void* a_scales, const void* w, const void* w_sca
     int device = 0, sms = 0;
     cudaGetDevice(&device);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    const int tiles = ((p.m + BM - 1) / BM) * ((p.n + BN - 1) / BN), pairs = tiles < sms / 2 ? tiles : sms / 2;
-    ti_launch_pdl(kernel, 2 * pairs, THREADS, T::SMEM, (cudaStream_t)stream, map_a, map_w, map_as, map_ws, p);
+    const int tiles = ((p.m + 255) / 256) * ((p.n + 255) / 256), pairs = tiles < sms / 2 ? tiles : sms / 2;
+    ti_launch_pdl(kernel, 2 * pairs, THREADS, T::SMEM, (cudaStream_t)stream, GLU ? map_a : map_w, GLU ? map_w : map_a,
+                  GLU ? map_as : map_ws, GLU ? map_ws : map_as, p);
     return ti_check_launch("mx_gemm_pairs");
 }
 
@@ -341,13 +354,14 @@ int launch(const void* a, const void* a_scales, const void* w, const void* w_sca
 // as ti_mx_gemm and ti_mx_gemm_glu (mx_gemm.cu), whose checks these run behind
 int mx_gemm_pairs(const void* a, const void* a_scales, int a_bits, const void* w, const void* w_scales, float* c, int m, int n,
                   int kp, int ldc, int accumulate, int settled, int* status, void* stream) {
-    const Args p{c, nullptr, nullptr, m, n, kp, ldc, 0, accumulate ? MODE_ACCUMULATE : MODE_STORE, settled, status};
-    return a_bits == 4 ? launch<4, 8>(a, a_scales, w, w_scales, p, stream) : launch<8, 8>(a, a_scales, w, w_scales, p, stream);
+    const Args p{c, nullptr, nullptr, m, n, kp, ldc, 0, accumulate, settled, status};
+    return a_bits == 4 ? launch<4, 8, false>(a, a_scales, w, w_scales, p, stream)
+                       : launch<8, 8, false>(a, a_scales, w, w_scales, p, stream);
 }
 int mx_gemm_pairs_glu(const void* a, const void* a_scales, int a_bits, const void* w, const void* w_scales, void* codes,
                       void* scales, int out_bits, int m, int out_kp, int kp, int settled, int* status, void* stream) {
-    const Args p{nullptr, (unsigned char*)codes, (unsigned char*)scales, m, 2 * out_kp, kp, 0, out_kp, MODE_GLU, settled, status};
-    if (out_bits == 8)
-        return a_bits == 4 ? launch<4, 8>(a, a_scales, w, w_scales, p, stream) : launch<8, 8>(a, a_scales, w, w_scales, p, stream);
-    return a_bits == 4 ? launch<4, 4>(a, a_scales, w, w_scales, p, stream) : launch<8, 4>(a, a_scales, w, w_scales, p, stream);
+    const Args p{nullptr, (unsigned char*)codes, (unsigned char*)scales, m, 2 * out_kp, kp, 0, out_kp, 0, settled, status};
+    auto run = out_bits == 8 ? (a_bits == 4 ? launch<4, 8, true> : launch<8, 8, true>)
+                             : (a_bits == 4 ? launch<4, 4, true> : launch<8, 4, true>);
+    return run(a, a_scales, w, w_scales, p, stream);
 }

@@ -1,10 +1,14 @@
 // Rows into the microscaled format (mx.cuh), out of it, and the root-mean-square norm whose output is in it.
 //
-// All three are bound by the bytes they move and, for few rows, by one round trip to memory.  A thread owns eight
-// neighbouring elements (16 bytes of bfloat16, 32 of float32), so a block of 32 is four lanes and a chunk of 128 sixteen:
-// the block's largest magnitude is two shuffles, a chunk's four scale bytes meet in one lane, which stores them as a word.
-// Rows whose start or stride does not allow such loads take a second form in which a warp walks a block with one element a
-// lane: every load is still 32 neighbours, the maximum is one redux.
+// All three are bound by the bytes they move and, for few rows, by one round trip to memory; the first two come close to the
+// limit of instructions too, so a thread's place costs no division (a block is a power of two of threads along a row) and
+// conversions are the hardware's, two elements each.  A thread owns eight neighbouring elements at a time (16 bytes of
+// bfloat16, 32 of float32), so a block of 32 is four lanes and a chunk of 128 sixteen: the block's largest magnitude is two
+// shuffles, a chunk's four scale bytes meet in one lane, which stores them as a word.  Rows whose start or stride does not
+// allow such accesses take a second form in which a warp walks a chunk with one element of each of its blocks a lane: every
+// access is still 32 neighbours, the maximum is one redux.
+#include <cuda_fp16.h>
+
 #include "mx.cuh"
 
 namespace {
@@ -61,58 +65,84 @@ template <typename T> __device__ __forceinline__ void store_guarded(T* row, int 
     }
 }
 
-// Codes and scales of a thread's eight elements at column c of a row; whole groups of sixteen neighbouring lanes call it
-// together, c a multiple of 128 in the group's first lane.
-template <int BITS>
-__device__ __forceinline__ void store_codes(const float (&v)[UNIT], int row, int c, int kp, unsigned char* codes,
-                                            unsigned char* scales) {
-    unsigned top = 0;
+// The largest magnitude's float32 bits.  Bits, not numbers: a NaN is larger than everything then.
+__device__ __forceinline__ unsigned top_of(const float (&v)[UNIT]) {
+    unsigned b[UNIT];
 #pragma unroll
-    for (int i = 0; i < UNIT; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    for (int i = 0; i < UNIT; ++i) b[i] = __float_as_uint(v[i]) & 0x7fffffffu;
+    const unsigned x = __vimax3_u32(b[0], b[1], b[2]), y = __vimax3_u32(b[3], b[4], b[5]);
+    return max(__vimax3_u32(x, y, b[6]), b[7]);
+}
+
+// Codes and scales of a thread's eight elements at column c of a row; whole groups of sixteen neighbouring lanes call it
+// together, c a multiple of 128 in the group's first lane.  `at`, `scale_word`: where the row's codes and the scale words of
+// its chunks begin (a row's words are 512 bytes apart).
+template <int BITS>
+__device__ __forceinline__ void store_codes(const float (&v)[UNIT], int c, unsigned char* at, unsigned char* scale_words) {
     const unsigned half = 0xffffu << (threadIdx.x & 16);
+    unsigned top = top_of(v);
     top = max(top, __shfl_xor_sync(half, top, 1));
     top = max(top, __shfl_xor_sync(half, top, 2));
     const unsigned s = scale_byte<BITS>(top);
     const float inv = scale_inverse(s);
-    unsigned char* at = codes + ((size_t)row * kp + c) / (8 / BITS);
     if (BITS == 8) {
         unsigned w[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             w[i] = codes_e4m3x2(v[4 * i] * inv, v[4 * i + 1] * inv) | codes_e4m3x2(v[4 * i + 2] * inv, v[4 * i + 3] * inv) << 16;
-        *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(at + c) = make_uint2(w[0], w[1]);
     } else {
         unsigned w = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) w |= codes_e2m1x2(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
-        *reinterpret_cast<unsigned*>(at) = w;
+        *reinterpret_cast<unsigned*>(at + c / 2) = w;
     }
     unsigned word = s << (8 * (threadIdx.x >> 2 & 3));       // the four blocks of a chunk: lanes 0, 4, 8, 12 of sixteen
     word |= __shfl_xor_sync(half, word, 4);
     word |= __shfl_xor_sync(half, word, 8);
-    if ((threadIdx.x & 15) == 0) *reinterpret_cast<unsigned*>(scales + scale_at(row, c / BLOCK, kp / CHUNK)) = word;
+    if ((threadIdx.x & 15) == 0) *reinterpret_cast<unsigned*>(scale_words + (size_t)(c / CHUNK) * TILE_BYTES) = word;
 }
 
 // ---- quantisation --------------------------------------------------------------------------------
 
 constexpr int QUANT_THREADS = 256;
+constexpr int AHEAD = 2;                // units of a thread, all asked for before the first is used
+
+// Where a thread of a row kernel works: 1 << shift threads lie along a row, QUANT_THREADS >> shift rows are in a block, and
+// blockIdx.y counts segments of AHEAD << shift units of a row.
+struct Place {
+    long long row;
+    int unit;                           // the first; the others follow at distances of 1 << shift
+    __device__ explicit Place(int shift)
+        : row(((long long)blockIdx.x << (8 - shift)) + (threadIdx.x >> shift)),
+          unit((int)((blockIdx.y * AHEAD) << shift) + ((int)threadIdx.x & ((1 << shift) - 1))) {}
+};
 
 template <typename T, int BITS>
 __global__ void __launch_bounds__(QUANT_THREADS)
-mx_quantize_kernel(const T* x, long long ld, int rows, int k, int kp, unsigned char* codes, unsigned char* scales) {
-    const unsigned per_row = (unsigned)kp / UNIT, at = blockIdx.x * QUANT_THREADS + threadIdx.x;
+mx_quantize_kernel(const T* x, long long ld, int rows, int k, int kp, unsigned char* codes, unsigned char* scales, int shift) {
+    const Place me(shift);
     pdl_wait();
-    if (at >= (unsigned)rows * per_row) return;              // whole groups of sixteen lanes: per_row is a multiple of 16
-    const int row = (int)(at / per_row), c = (int)(at % per_row) * UNIT;
-    float v[UNIT];
-    load_guarded(x + (size_t)row * ld, c, k, true, v);
-    store_codes<BITS>(v, row, c, kp, codes, scales);
+    if (me.row >= rows) return;                              // whole groups of sixteen lanes, here and below
+    const T* from = x + (size_t)me.row * ld;
+    float v[AHEAD][UNIT];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+        const int c = (me.unit + (u << shift)) * UNIT;
+        if (c < kp) load_guarded(from, c, k, true, v[u]);
+    }
+    unsigned char *at = codes + (size_t)me.row * kp / (8 / BITS), *words = scales + scale_at((int)me.row, 0, kp / CHUNK);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+        const int c = (me.unit + (u << shift)) * UNIT;
+        if (c < kp) store_codes<BITS>(v[u], c, at, words);
+    }
 }
 
 // any start and stride: a warp takes a chunk, one element of each of its four blocks a lane
 template <typename T, int BITS>
 __global__ void __launch_bounds__(QUANT_THREADS)
-mx_quantize_any_kernel(const T* x, long long ld, int rows, int k, int kp, unsigned char* codes, unsigned char* scales) {
+mx_quantize_any_kernel(const T* x, long long ld, int rows, int k, int kp, unsigned char* codes, unsigned char* scales, int) {
     const unsigned chunks = (unsigned)kp / CHUNK, at = (blockIdx.x * QUANT_THREADS + threadIdx.x) / 32;
     const int lane = threadIdx.x & 31;
     pdl_wait();
@@ -141,31 +171,74 @@ mx_quantize_any_kernel(const T* x, long long ld, int rows, int k, int kp, unsign
 
 // ---- and back ------------------------------------------------------------------------------------
 
+// eight codes as numbers without their scale; both element types are exact in float16
+template <int BITS> __device__ __forceinline__ void values_of(uint2 w, float (&v)[UNIT]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        unsigned pair;
+        if (BITS == 8)
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(pair) : "h"((unsigned short)((i < 2 ? w.x : w.y) >> (16 * (i & 1)))));
+        else
+            asm("{\n\t.reg .b8 b;\n\tcvt.u8.u32 b, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(pair) : "r"(w.x >> (8 * i)));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+
 template <typename T, int BITS>
 __global__ void __launch_bounds__(QUANT_THREADS)
 mx_dequantize_kernel(const unsigned char* codes, const unsigned char* scales, int rows, int k, int kp, T* out, long long ld,
-                     bool whole) {
-    const unsigned per_row = ((unsigned)k + UNIT - 1) / UNIT, at = blockIdx.x * QUANT_THREADS + threadIdx.x;
+                     int shift) {
+    const Place me(shift);
     pdl_launch();
     pdl_wait();
-    if (at >= (unsigned)rows * per_row) return;
-    const int row = (int)(at / per_row), c = (int)(at % per_row) * UNIT;
-    const unsigned char* from = codes + ((size_t)row * kp + c) / (8 / BITS);
-    const float f = scale_value(scales[scale_at(row, c / BLOCK, kp / CHUNK)]);
-    float v[UNIT];
-    if (BITS == 8) {
-        const uint2 w = *reinterpret_cast<const uint2*>(from);
+    if (me.row >= rows) return;
+    const unsigned char *at = codes + (size_t)me.row * kp / (8 / BITS), *words = scales + scale_at((int)me.row, 0, kp / CHUNK);
+    uint2 w[AHEAD];
+    unsigned s[AHEAD];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = value_e4m3(w.x >> (8 * i) & 255u) * f;
-            v[4 + i] = value_e4m3(w.y >> (8 * i) & 255u) * f;
+    for (int u = 0; u < AHEAD; ++u) {
+        const int c = (me.unit + (u << shift)) * UNIT;
+        if (c < k) {
+            w[u] = BITS == 8 ? *reinterpret_cast<const uint2*>(at + c) : make_uint2(*reinterpret_cast<const unsigned*>(at + c / 2), 0);
+            s[u] = words[(size_t)(c / CHUNK) * TILE_BYTES + c / BLOCK % 4];
         }
-    } else {
-        const unsigned w = *reinterpret_cast<const unsigned*>(from);
-#pragma unroll
-        for (int i = 0; i < UNIT; ++i) v[i] = value_e2m1(w >> (4 * i) & 15u) * f;
     }
-    store_guarded(out + (size_t)row * ld, c, k, whole, v);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+        const int c = (me.unit + (u << shift)) * UNIT;
+        if (c >= k) break;
+        const float f = scale_value(s[u]);
+        float v[UNIT];
+        values_of<BITS>(w[u], v);
+#pragma unroll
+        for (int i = 0; i < UNIT; ++i) v[i] *= f;
+        store_guarded(out + (size_t)me.row * ld, c, k, true, v);
+    }
+}
+
+// rows of the output off 16 bytes
+template <typename T, int BITS>
+__global__ void __launch_bounds__(QUANT_THREADS)
+mx_dequantize_any_kernel(const unsigned char* codes, const unsigned char* scales, int rows, int k, int kp, T* out, long long ld,
+                         int) {
+    const unsigned chunks = (unsigned)kp / CHUNK, at = (blockIdx.x * QUANT_THREADS + threadIdx.x) / 32;
+    const int lane = threadIdx.x & 31;
+    pdl_launch();
+    pdl_wait();
+    if (at >= (unsigned)rows * chunks) return;
+    const int row = (int)(at / chunks), c = (int)(at % chunks) * CHUNK;
+    const unsigned word = *reinterpret_cast<const unsigned*>(scales + scale_at(row, c / BLOCK, kp / CHUNK));
+    const unsigned char* from = codes + ((size_t)row * kp + c) / (8 / BITS);
+    T* to = out + (size_t)row * ld + c;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const int e = b * BLOCK + lane;
+        const unsigned code = BITS == 8 ? from[e] : from[e / 2] >> (4 * (lane & 1)) & 15u;
+        const float v = (BITS == 8 ? value_e4m3(code) : value_e2m1(code)) * scale_value(word >> (8 * b) & 255u);
+        if (c + e < k) to[e] = from_f32<T>(v);
+    }
 }
 
 // ---- the norm ------------------------------------------------------------------------------------
@@ -208,30 +281,49 @@ mx_rmsnorm_kernel(float* x, long long ldx, const D* delta, long long ldd, const 
         load_guarded(weight, c, k, whole_w, w);
 #pragma unroll
         for (int i = 0; i < UNIT; ++i) v[u][i] = v[u][i] * inv * w[i];
-        store_codes<BITS>(v[u], row, c, kp, codes, scales);
+        store_codes<BITS>(v[u], c, codes + (size_t)row * kp / (8 / BITS), scales + scale_at(row, 0, kp / CHUNK));
     }
 }
 
 bool whole_rows(const void* p, long long ld, int bytes) { return (uintptr_t)p % 16 == 0 && ld * bytes % 16 == 0; }
 
+// The launch of a row kernel over `units` of eight elements a row: as many threads along a row as its units want at AHEAD
+// each (16 to 256), or for rows off 16 bytes a warp a chunk.  False: too many for a grid.
+struct Shape {
+    dim3 grid;
+    int shift = 8;
+    bool set(bool whole, long long rows, int units, int chunks) {
+        if (!whole) {
+            const long long warps = rows * chunks;
+            grid = dim3((unsigned)((warps + QUANT_THREADS / 32 - 1) / (QUANT_THREADS / 32)));
+            return warps < (1LL << 27);
+        }
+        while (shift > 4 && AHEAD << (shift - 1) >= units) --shift;
+        const long long in_block = QUANT_THREADS >> shift, segments = (units + (AHEAD << shift) - 1) / (AHEAD << shift);
+        grid = dim3((unsigned)((rows + in_block - 1) / in_block), (unsigned)segments);
+        return segments < 65536;
+    }
+};
+
 template <typename T, int BITS>
 int quantize(const void* x, long long ld, int rows, int k, int kp, void* codes, void* scales, void* stream) {
     const bool whole = whole_rows(x, ld, sizeof(T));
-    const long long threads = whole ? (long long)rows * (kp / UNIT) : (long long)rows * (kp / CHUNK) * 32;
-    TI_REQUIRE(threads < (1LL << 32) - QUANT_THREADS, "mx_quantize: %d rows of %d elements are too many", rows, k);
-    const unsigned blocks = (unsigned)((threads + QUANT_THREADS - 1) / QUANT_THREADS);
-    ti_launch_pdl(whole ? mx_quantize_kernel<T, BITS> : mx_quantize_any_kernel<T, BITS>, blocks, QUANT_THREADS, 0,
-                  (cudaStream_t)stream, (const T*)x, ld, rows, k, kp, (unsigned char*)codes, (unsigned char*)scales);
+    Shape shape;
+    TI_REQUIRE(shape.set(whole, rows, kp / UNIT, kp / CHUNK), "mx_quantize: %d rows of %d elements are too many", rows, k);
+    ti_launch_pdl(whole ? mx_quantize_kernel<T, BITS> : mx_quantize_any_kernel<T, BITS>, shape.grid, QUANT_THREADS, 0,
+                  (cudaStream_t)stream, (const T*)x, ld, rows, k, kp, (unsigned char*)codes, (unsigned char*)scales, shape.shift);
     return ti_check_launch("mx_quantize");
 }
 
 template <typename T, int BITS>
 int dequantize(const void* codes, const void* scales, int rows, int k, int kp, void* out, long long ld, void* stream) {
-    const long long threads = (long long)rows * ((k + UNIT - 1) / UNIT);
-    TI_REQUIRE(threads < (1LL << 32) - QUANT_THREADS, "mx_dequantize: %d rows of %d elements are too many", rows, k);
-    ti_launch_pdl(mx_dequantize_kernel<T, BITS>, (unsigned)((threads + QUANT_THREADS - 1) / QUANT_THREADS), QUANT_THREADS, 0,
+    const bool whole = whole_rows(out, ld, sizeof(T));
+    Shape shape;
+    TI_REQUIRE(shape.set(whole, rows, (k + UNIT - 1) / UNIT, kp / CHUNK), "mx_dequantize: %d rows of %d elements are too many",
+               rows, k);
+    ti_launch_pdl(whole ? mx_dequantize_kernel<T, BITS> : mx_dequantize_any_kernel<T, BITS>, shape.grid, QUANT_THREADS, 0,
                   (cudaStream_t)stream, (const unsigned char*)codes, (const unsigned char*)scales, rows, k, kp, (T*)out, ld,
-                  whole_rows(out, ld, sizeof(T)));
+                  shape.shift);
     return ti_check_launch("mx_dequantize");
 }
 

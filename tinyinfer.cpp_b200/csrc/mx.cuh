@@ -39,15 +39,29 @@ __device__ __forceinline__ float scale_value(unsigned s) {
     return __uint_as_float(s == 255 ? 0x7fffffffu : s == 0 ? 0x00400000u : s << 23);
 }
 
-// two neighbours' codes: e4m3 in the low 16 bits, e2m1 in the low 8 (the first element low)
+// codes of neighbours, the first one lowest: one in the low bits, four e4m3 or eight e2m1 as a word
 __device__ __forceinline__ unsigned codes_e4m3x2(float first, float second) {
     unsigned short r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(second), "f"(first));
     return r;
 }
+__device__ __forceinline__ unsigned codes_e4m3x4(const float* y) {
+    unsigned r;
+    asm("{\n\t.reg .b16 a, b;\n\tcvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\t"
+        "mov.b32 %0, {a, b};\n\t}" : "=r"(r) : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]));
+    return r;
+}
 __device__ __forceinline__ unsigned codes_e2m1x2(float first, float second) {
     unsigned r;
-    asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\tcvt.u32.u8 %0, b;\n\t}" : "=r"(r) : "f"(second), "f"(first));
+    asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\tcvt.u32.u8 %0, b;\n\t}"
+        : "=r"(r) : "f"(second), "f"(first));
+    return r;
+}
+__device__ __forceinline__ unsigned codes_e2m1x8(const float* y) {
+    unsigned r;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r) : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
     return r;
 }
 // the value of one code

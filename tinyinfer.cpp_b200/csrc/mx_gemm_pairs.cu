@@ -109,14 +109,9 @@ __device__ __forceinline__ void finish_glu(const Args& p, const unsigned* gate, 
     unsigned char* at = p.out_codes + ((size_t)row * p.out_kp + out_col) / (8 / OBITS);
     unsigned w[OBITS];
 #pragma unroll
-    for (int i = 0; i < OBITS; ++i) {
-        w[i] = 0;
+    for (int i = 0; i < 32; ++i) h[i] *= inv;
 #pragma unroll
-        for (int j = 0; j < 32 / OBITS; j += 2) {
-            const float a = h[i * (32 / OBITS) + j] * inv, b = h[i * (32 / OBITS) + j + 1] * inv;
-            w[i] |= (OBITS == 8 ? codes_e4m3x2(a, b) : codes_e2m1x2(a, b)) << (OBITS * j);
-        }
-    }
+    for (int i = 0; i < OBITS; ++i) w[i] = OBITS == 8 ? codes_e4m3x4(h + 4 * i) : codes_e2m1x8(h + 8 * i);
 #pragma unroll
     for (int i = 0; i < OBITS; i += 4)
         *reinterpret_cast<uint4*>(at + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);

@@ -4,9 +4,9 @@
 // limit of instructions too, so a thread's place costs no division (a block is a power of two of threads along a row) and
 // conversions are the hardware's, two elements each.  A thread owns eight neighbouring elements at a time (16 bytes of
 // bfloat16, 32 of float32), so a block of 32 is four lanes and a chunk of 128 sixteen: the block's largest magnitude is two
-// shuffles, a chunk's four scale bytes meet in one lane, which stores them as a word.  Rows whose start or stride does not
-// allow such accesses take a second form in which a warp walks a chunk with one element of each of its blocks a lane: every
-// access is still 32 neighbours, the maximum is one redux.
+// shuffles, a chunk's four scale bytes meet in one lane, which stores them as a word.  Rows whose start, stride or length does
+// not allow such accesses are read element by element (the lines come from L1) and written by warps that walk a chunk with
+// one element of each of its blocks a lane.
 #include <cuda_fp16.h>
 
 #include "mx.cuh"
@@ -17,9 +17,7 @@ using namespace mx;
 
 constexpr int UNIT = 8;                 // elements of a thread
 
-template <typename T> __device__ __forceinline__ void load_unit(const T* p, float (&v)[UNIT]);
-template <> __device__ __forceinline__ void load_unit<bf16>(const bf16* p, float (&v)[UNIT]) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void widen(const uint4& raw, float (&v)[UNIT]) {
     const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -27,7 +25,8 @@ template <> __device__ __forceinline__ void load_unit<bf16>(const bf16* p, float
         v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
 }
-template <> __device__ __forceinline__ void load_unit<float>(const float* p, float (&v)[UNIT]) {
+__device__ __forceinline__ void load_unit(const bf16* p, float (&v)[UNIT]) { widen(*reinterpret_cast<const uint4*>(p), v); }
+__device__ __forceinline__ void load_unit(const float* p, float (&v)[UNIT]) {
     const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
@@ -65,108 +64,119 @@ template <typename T> __device__ __forceinline__ void store_guarded(T* row, int 
     }
 }
 
-// The largest magnitude's float32 bits.  Bits, not numbers: a NaN is larger than everything then.
+// The largest magnitude's float32 bits, over the thread's elements and over its block's.  Bits, not numbers: a NaN is larger
+// than everything then.
+__device__ __forceinline__ unsigned top_of_block(unsigned top) {
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    return max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+}
 __device__ __forceinline__ unsigned top_of(const float (&v)[UNIT]) {
     unsigned b[UNIT];
 #pragma unroll
     for (int i = 0; i < UNIT; ++i) b[i] = __float_as_uint(v[i]) & 0x7fffffffu;
     const unsigned x = __vimax3_u32(b[0], b[1], b[2]), y = __vimax3_u32(b[3], b[4], b[5]);
-    return max(__vimax3_u32(x, y, b[6]), b[7]);
+    return top_of_block(max(__vimax3_u32(x, y, b[6]), b[7]));
+}
+// ... of eight bfloat16 as they were loaded: two at a time
+__device__ __forceinline__ unsigned top_of(const uint4& raw) {
+    unsigned t = __vmaxu2(__vmaxu2(raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu), __vmaxu2(raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu));
+    t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, 1));
+    t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, 2));
+    return max(t & 0xffff0000u, t << 16);
 }
 
-// Codes and scales of a thread's eight elements at column c of a row; whole groups of sixteen neighbouring lanes call it
-// together, c a multiple of 128 in the group's first lane.  `at`, `scale_word`: where the row's codes and the scale words of
-// its chunks begin (a row's words are 512 bytes apart).
+// Codes and scales of a thread's eight elements at column c of a row, `top` their block's largest magnitude, c a multiple of 128 in the first of sixteen lanes.  A
+// whole warp calls it (shuffles under a mask that is not known when compiling cost far more), lanes with nothing to store
+// with `valid` false.  `at`, `scale_words`: where the row's codes and the scale words of its chunks begin (a row's words are
+// 512 bytes apart).
 template <int BITS>
-__device__ __forceinline__ void store_codes(const float (&v)[UNIT], int c, unsigned char* at, unsigned char* scale_words) {
-    const unsigned half = 0xffffu << (threadIdx.x & 16);
-    unsigned top = top_of(v);
-    top = max(top, __shfl_xor_sync(half, top, 1));
-    top = max(top, __shfl_xor_sync(half, top, 2));
+__device__ __forceinline__ void store_codes(const float (&v)[UNIT], unsigned top, int c, bool valid, unsigned char* at,
+                                            unsigned char* scale_words) {
     const unsigned s = scale_byte<BITS>(top);
     const float inv = scale_inverse(s);
+    float y[UNIT];
+#pragma unroll
+    for (int i = 0; i < UNIT; ++i) y[i] = v[i] * inv;
     if (BITS == 8) {
-        unsigned w[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            w[i] = codes_e4m3x2(v[4 * i] * inv, v[4 * i + 1] * inv) | codes_e4m3x2(v[4 * i + 2] * inv, v[4 * i + 3] * inv) << 16;
-        *reinterpret_cast<uint2*>(at + c) = make_uint2(w[0], w[1]);
+        const uint2 w = make_uint2(codes_e4m3x4(y), codes_e4m3x4(y + 4));
+        if (valid) *reinterpret_cast<uint2*>(at + c) = w;
     } else {
-        unsigned w = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w |= codes_e2m1x2(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
-        *reinterpret_cast<unsigned*>(at + c / 2) = w;
+        const unsigned w = codes_e2m1x8(y);
+        if (valid) *reinterpret_cast<unsigned*>(at + c / 2) = w;
     }
     unsigned word = s << (8 * (threadIdx.x >> 2 & 3));       // the four blocks of a chunk: lanes 0, 4, 8, 12 of sixteen
-    word |= __shfl_xor_sync(half, word, 4);
-    word |= __shfl_xor_sync(half, word, 8);
-    if ((threadIdx.x & 15) == 0) *reinterpret_cast<unsigned*>(scale_words + (size_t)(c / CHUNK) * TILE_BYTES) = word;
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    if (valid && (threadIdx.x & 15) == 0) *reinterpret_cast<unsigned*>(scale_words + (size_t)(c / CHUNK) * TILE_BYTES) = word;
 }
 
 // ---- quantisation --------------------------------------------------------------------------------
 
 constexpr int QUANT_THREADS = 256;
-constexpr int AHEAD = 2;                // units of a thread, all asked for before the first is used
 
 // Where a thread of a row kernel works: 1 << shift threads lie along a row, QUANT_THREADS >> shift rows are in a block, and
-// blockIdx.y counts segments of AHEAD << shift units of a row.
+// blockIdx.y counts segments of `ahead` << shift units of a row, `ahead` of them a thread's, all asked for before the first
+// is used.
 struct Place {
     long long row;
     int unit;                           // the first; the others follow at distances of 1 << shift
-    __device__ explicit Place(int shift)
+    __device__ Place(int shift, int ahead)
         : row(((long long)blockIdx.x << (8 - shift)) + (threadIdx.x >> shift)),
-          unit((int)((blockIdx.y * AHEAD) << shift) + ((int)threadIdx.x & ((1 << shift) - 1))) {}
+          unit((int)((blockIdx.y * ahead) << shift) + ((int)threadIdx.x & ((1 << shift) - 1))) {}
 };
 
-template <typename T, int BITS>
+// Eight elements as they were loaded, then as numbers with their block's top.  `held` of them are inside the row; WHOLE: all
+// or none, on 16 bytes.
+template <typename T, bool WHOLE> struct Unit {
+    float v[UNIT];
+    __device__ void load(const T* p, int held) {
+        if (WHOLE) {
+            if (held > 0) {
+                load_unit(p, v);
+                return;
+            }
+            held = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < UNIT; ++i) v[i] = i < held ? to_f32(p[i]) : 0.0f;
+    }
+    __device__ unsigned take(float (&out)[UNIT]) const {
+#pragma unroll
+        for (int i = 0; i < UNIT; ++i) out[i] = v[i];
+        return top_of(v);
+    }
+};
+template <> struct Unit<bf16, true> {
+    uint4 raw;
+    __device__ void load(const bf16* p, int held) {
+        raw = held > 0 ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+    }
+    __device__ unsigned take(float (&out)[UNIT]) const {
+        widen(raw, out);
+        return top_of(raw);
+    }
+};
+
+template <typename T, int BITS, bool WHOLE, int AHEAD>
 __global__ void __launch_bounds__(QUANT_THREADS)
 mx_quantize_kernel(const T* x, long long ld, int rows, int k, int kp, unsigned char* codes, unsigned char* scales, int shift) {
-    const Place me(shift);
+    const Place me(shift, AHEAD);
     pdl_wait();
-    if (me.row >= rows) return;                              // whole groups of sixteen lanes, here and below
     const T* from = x + (size_t)me.row * ld;
-    float v[AHEAD][UNIT];
+    Unit<T, WHOLE> units[AHEAD];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
         const int c = (me.unit + (u << shift)) * UNIT;
-        if (c < kp) load_guarded(from, c, k, true, v[u]);
+        units[u].load(from + c, me.row < rows ? k - c : 0);
     }
     unsigned char *at = codes + (size_t)me.row * kp / (8 / BITS), *words = scales + scale_at((int)me.row, 0, kp / CHUNK);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
         const int c = (me.unit + (u << shift)) * UNIT;
-        if (c < kp) store_codes<BITS>(v[u], c, at, words);
+        float v[UNIT];
+        const unsigned top = units[u].take(v);
+        store_codes<BITS>(v, top, c, me.row < rows && c < kp, at, words);
     }
-}
-
-// any start and stride: a warp takes a chunk, one element of each of its four blocks a lane
-template <typename T, int BITS>
-__global__ void __launch_bounds__(QUANT_THREADS)
-mx_quantize_any_kernel(const T* x, long long ld, int rows, int k, int kp, unsigned char* codes, unsigned char* scales, int) {
-    const unsigned chunks = (unsigned)kp / CHUNK, at = (blockIdx.x * QUANT_THREADS + threadIdx.x) / 32;
-    const int lane = threadIdx.x & 31;
-    pdl_wait();
-    if (at >= (unsigned)rows * chunks) return;
-    const int row = (int)(at / chunks), c = (int)(at % chunks) * CHUNK;
-    const T* from = x + (size_t)row * ld;
-    float v[4];
-#pragma unroll
-    for (int b = 0; b < 4; ++b) v[b] = c + b * BLOCK + lane < k ? to_f32(from[c + b * BLOCK + lane]) : 0.0f;
-    unsigned word = 0;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        const unsigned s = scale_byte<BITS>(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7fffffffu));
-        word |= s << (8 * b);
-        const float y = v[b] * scale_inverse(s);
-        const size_t el = (size_t)row * kp + c + b * BLOCK + lane;
-        if (BITS == 8) {
-            codes[el] = (unsigned char)codes_e4m3x2(y, 0.0f);
-        } else {
-            const float next = __shfl_down_sync(0xffffffffu, y, 1);
-            if (!(lane & 1)) codes[el / 2] = (unsigned char)codes_e2m1x2(y, next);
-        }
-    }
-    if (lane == 0) *reinterpret_cast<unsigned*>(scales + scale_at(row, c / BLOCK, kp / CHUNK)) = word;
 }
 
 // ---- and back ------------------------------------------------------------------------------------
@@ -186,11 +196,11 @@ template <int BITS> __device__ __forceinline__ void values_of(uint2 w, float (&v
     }
 }
 
-template <typename T, int BITS>
+template <typename T, int BITS, int AHEAD>
 __global__ void __launch_bounds__(QUANT_THREADS)
 mx_dequantize_kernel(const unsigned char* codes, const unsigned char* scales, int rows, int k, int kp, T* out, long long ld,
                      int shift) {
-    const Place me(shift);
+    const Place me(shift, AHEAD);
     pdl_launch();
     pdl_wait();
     if (me.row >= rows) return;
@@ -214,7 +224,7 @@ mx_dequantize_kernel(const unsigned char* codes, const unsigned char* scales, in
         values_of<BITS>(w[u], v);
 #pragma unroll
         for (int i = 0; i < UNIT; ++i) v[i] *= f;
-        store_guarded(out + (size_t)me.row * ld, c, k, true, v);
+        store_unit(out + (size_t)me.row * ld + c, v);         // k is a multiple of 8
     }
 }
 
@@ -276,54 +286,55 @@ mx_rmsnorm_kernel(float* x, long long ldx, const D* delta, long long ldd, const 
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
         const int c = (u * (int)blockDim.x + (int)threadIdx.x) * UNIT;
-        if (c >= kp) break;                                  // whole groups of sixteen lanes: kp is a multiple of 128
         float w[UNIT];
         load_guarded(weight, c, k, whole_w, w);
 #pragma unroll
         for (int i = 0; i < UNIT; ++i) v[u][i] = v[u][i] * inv * w[i];
-        store_codes<BITS>(v[u], c, codes + (size_t)row * kp / (8 / BITS), scales + scale_at(row, 0, kp / CHUNK));
+        store_codes<BITS>(v[u], top_of(v[u]), c, c < kp, codes + (size_t)row * kp / (8 / BITS), scales + scale_at(row, 0, kp / CHUNK));
     }
 }
 
 bool whole_rows(const void* p, long long ld, int bytes) { return (uintptr_t)p % 16 == 0 && ld * bytes % 16 == 0; }
 
-// The launch of a row kernel over `units` of eight elements a row: as many threads along a row as its units want at AHEAD
-// each (16 to 256), or for rows off 16 bytes a warp a chunk.  False: too many for a grid.
+// The launch of a row kernel over `units` of eight elements a row: as many threads along a row as its units want (16 to 256).
+// Four units a thread where the GPU (148 SMs of 2,048 threads) is full all the same, else one: 12,288 x 4,096 bfloat16 into 4
+// bits and back 31.7 + 30.9 us with one, 27.0 + 23.5 with two, 24.0 + 21.2 with four; 8 x 4,096 1.38 us with one, 1.85 with two.
 struct Shape {
     dim3 grid;
-    int shift = 8;
-    bool set(bool whole, long long rows, int units, int chunks) {
-        if (!whole) {
-            const long long warps = rows * chunks;
-            grid = dim3((unsigned)((warps + QUANT_THREADS / 32 - 1) / (QUANT_THREADS / 32)));
-            return warps < (1LL << 27);
-        }
-        while (shift > 4 && AHEAD << (shift - 1) >= units) --shift;
-        const long long in_block = QUANT_THREADS >> shift, segments = (units + (AHEAD << shift) - 1) / (AHEAD << shift);
+    int shift = 8, ahead;
+    Shape(long long rows, int units) : ahead(rows * units >= 4LL * 148 * 2048 ? 4 : 1) {
+        while (shift > 4 && ahead << (shift - 1) >= units) --shift;
+        const long long in_block = QUANT_THREADS >> shift, segments = (units + (ahead << shift) - 1) / (ahead << shift);
         grid = dim3((unsigned)((rows + in_block - 1) / in_block), (unsigned)segments);
-        return segments < 65536;
     }
 };
 
 template <typename T, int BITS>
 int quantize(const void* x, long long ld, int rows, int k, int kp, void* codes, void* scales, void* stream) {
-    const bool whole = whole_rows(x, ld, sizeof(T));
-    Shape shape;
-    TI_REQUIRE(shape.set(whole, rows, kp / UNIT, kp / CHUNK), "mx_quantize: %d rows of %d elements are too many", rows, k);
-    ti_launch_pdl(whole ? mx_quantize_kernel<T, BITS> : mx_quantize_any_kernel<T, BITS>, shape.grid, QUANT_THREADS, 0,
-                  (cudaStream_t)stream, (const T*)x, ld, rows, k, kp, (unsigned char*)codes, (unsigned char*)scales, shape.shift);
+    const bool whole = whole_rows(x, ld, sizeof(T)) && k % UNIT == 0;
+    const Shape shape(rows, kp / UNIT);
+    TI_REQUIRE(shape.grid.y < 65536, "mx_quantize: rows of %d elements are too long", k);
+    auto kernel = shape.ahead == 4 ? (whole ? mx_quantize_kernel<T, BITS, true, 4> : mx_quantize_kernel<T, BITS, false, 4>)
+                                   : (whole ? mx_quantize_kernel<T, BITS, true, 1> : mx_quantize_kernel<T, BITS, false, 1>);
+    ti_launch_pdl(kernel, shape.grid, QUANT_THREADS, 0, (cudaStream_t)stream, (const T*)x, ld, rows, k, kp, (unsigned char*)codes,
+                  (unsigned char*)scales, shape.shift);
     return ti_check_launch("mx_quantize");
 }
 
 template <typename T, int BITS>
 int dequantize(const void* codes, const void* scales, int rows, int k, int kp, void* out, long long ld, void* stream) {
-    const bool whole = whole_rows(out, ld, sizeof(T));
-    Shape shape;
-    TI_REQUIRE(shape.set(whole, rows, (k + UNIT - 1) / UNIT, kp / CHUNK), "mx_dequantize: %d rows of %d elements are too many",
-               rows, k);
-    ti_launch_pdl(whole ? mx_dequantize_kernel<T, BITS> : mx_dequantize_any_kernel<T, BITS>, shape.grid, QUANT_THREADS, 0,
-                  (cudaStream_t)stream, (const unsigned char*)codes, (const unsigned char*)scales, rows, k, kp, (T*)out, ld,
-                  shape.shift);
+    const bool whole = whole_rows(out, ld, sizeof(T)) && k % UNIT == 0;
+    Shape shape(rows, (k + UNIT - 1) / UNIT);
+    auto kernel = shape.ahead == 4 ? mx_dequantize_kernel<T, BITS, 4> : mx_dequantize_kernel<T, BITS, 1>;
+    if (!whole) {                                            // a warp a chunk
+        const long long warps = (long long)rows * (kp / CHUNK);
+        TI_REQUIRE(warps < (1LL << 27), "mx_dequantize: %d rows of %d elements are too many", rows, k);
+        shape.grid = dim3((unsigned)((warps + QUANT_THREADS / 32 - 1) / (QUANT_THREADS / 32)));
+        kernel = mx_dequantize_any_kernel<T, BITS>;
+    }
+    TI_REQUIRE(shape.grid.y < 65536, "mx_dequantize: rows of %d elements are too long", k);
+    ti_launch_pdl(kernel, shape.grid, QUANT_THREADS, 0, (cudaStream_t)stream, (const unsigned char*)codes,
+                  (const unsigned char*)scales, rows, k, kp, (T*)out, ld, shape.shift);
     return ti_check_launch("mx_dequantize");
 }
 

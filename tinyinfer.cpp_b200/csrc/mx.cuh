@@ -64,19 +64,6 @@ __device__ __forceinline__ unsigned codes_e2m1x8(const float* y) {
         : "=r"(r) : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
     return r;
 }
-// the value of one code
-__device__ __forceinline__ float value_e4m3(unsigned c) {
-    // exponent and mantissa moved to float16's places give value / 2^8; e = 15 with mantissa 7 is NaN
-    if ((c & 0x7f) == 0x7f) return __uint_as_float(0x7fffffffu);
-    const unsigned mag = c & 0x7f;
-    const float v = mag >= 8 ? __uint_as_float((mag << 20) + (120u << 23)) : (float)mag * 0.001953125f;
-    return c & 0x80 ? -v : v;
-}
-__device__ __forceinline__ float value_e2m1(unsigned c) {
-    const unsigned mag = c & 7;
-    const float v = mag >= 2 ? __uint_as_float((mag << 22) + (126u << 23)) : (float)mag * 0.5f;
-    return c & 8 ? -v : v;
-}
 
 // ---- clusters ------------------------------------------------------------------------------------
 

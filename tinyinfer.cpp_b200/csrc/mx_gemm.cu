@@ -197,7 +197,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         // a stage's scale tiles into the stage's columns: W's four, then four per tile of A, per chunk
         for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
             const int s = it % STAGES, held = min(CHUNKS, chunks - kb * CHUNKS);
-            ok = mbar_wait(&scales_full[s], (it / STAGES) & 1);
+            ok = __all_sync(0xffffffffu, mbar_wait(&scales_full[s], (it / STAGES) & 1));
             if (!ok) break;
             const uint4* from = reinterpret_cast<const uint4*>(stage_s + s * T::STAGE_S) + lane;
             for (int j = 0; j < held; ++j)
@@ -210,7 +210,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             if (lane == 0) mbar_arrive(&scaled[s]);
         }
         pdl_wait();                                           // C belongs to the chain of launches
-        ok = ok && mbar_wait(acc_full, 0);
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_full, 0));
         tc_fence_after();
         const int held_tok = min(NTOK, p.m - tok0);
         if (p.mode != MODE_GLU && p.parts == 1) {             // straight to C: a warp's lanes are 32 neighbouring columns

@@ -251,7 +251,7 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
             const int mine = num_tiles > pair ? (num_tiles - pair + num_pairs - 1) / num_pairs : 0;
             for (int it = 0; it < mine * num_kb; ++it) {
                 const int s = it % STAGES;
-                ok = mbar_wait(&scales_full[s], (it / STAGES) & 1);
+                ok = __all_sync(0xffffffffu, mbar_wait(&scales_full[s], (it / STAGES) & 1));
                 if (!ok) break;
                 const uint4* from = reinterpret_cast<const uint4*>(stage_s + s * 3 * T::SCALES) + lane;
 #pragma unroll
@@ -272,7 +272,7 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
         int local = 0;
         for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local) {
             const int tok0 = tile % tiles_a * 256, n0 = tile / tiles_a * 256, mine = (int)rank * 128 + quarter * 32 + lane;
-            ok = mbar_wait(acc_full, local & 1);
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full, local & 1));
             if (!ok) break;
             tc_fence_after();
             unsigned v[128];

@@ -31,17 +31,15 @@ enum { TI_ERR_TIMEOUT = 2 };
 template <int NTOK, int ABITS> struct Tile {
     static constexpr int ELEMS = ABITS == 4 ? 256 : 128;                 // of K in a stage
     static constexpr int CHUNKS = ELEMS / CHUNK;
-    static constexpr int XTILES = (NTOK + TILE_ROWS - 1) / TILE_ROWS;     // scale tiles of A per chunk
-    static constexpr int STAGE_W = BW * ROW, STAGE_X = NTOK * ROW;
-    static constexpr int STAGE_S = CHUNKS * (1 + XTILES) * TILE_BYTES;
-    static constexpr int PER_SM = NTOK <= 128 ? 2 : 1;                    // blocks of an SM
-    static constexpr int STAGES = NTOK == 256 ? 4 : NTOK == 128 ? 3 : NTOK == 64 ? 4 : 5;
+    static constexpr int STAGE_W = BW * ROW, STAGE_X = NTOK * ROW, STAGE_S = CHUNKS * 2 * TILE_BYTES;
+    static constexpr int PER_SM = 2;                                      // blocks of an SM
+    static constexpr int STAGES = NTOK == 128 ? 3 : NTOK == 64 ? 4 : 5;
     static constexpr int SMEM = STAGES * (STAGE_W + STAGE_X + STAGE_S) + 1024 + 256;
-    static constexpr int SCALE_COLS = CHUNKS * 4 * (1 + XTILES);          // tensor memory columns of a stage's scales
+    static constexpr int SCALE_COLS = CHUNKS * 8;                         // tensor memory columns of a stage's scales
     static constexpr int ACC_COLS = NTOK < 32 ? 32 : NTOK;
     static constexpr int COLS = ACC_COLS + STAGES * SCALE_COLS;
-    static constexpr unsigned TMEM_COLS = COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
-    static_assert(COLS <= 512 && TMEM_COLS * PER_SM <= 512, "tensor memory");
+    static constexpr unsigned TMEM_COLS = COLS <= 128 ? 128 : 256;
+    static_assert(COLS <= 256, "tensor memory");
     static_assert(SMEM * PER_SM <= 227 * 1024, "shared memory");
     static_assert(STAGES * (STAGE_W + STAGE_X) >= NTOK * BW * 4, "the sums of a tile have to fit where the stages were");
 };
@@ -101,7 +99,7 @@ template <int NTOK, int ABITS, int OBITS>
 __global__ void __launch_bounds__(THREADS)
 mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Args p) {
     using T = Tile<NTOK, ABITS>;
-    constexpr int STAGES = T::STAGES, CHUNKS = T::CHUNKS, XTILES = T::XTILES;
+    constexpr int STAGES = T::STAGES, CHUNKS = T::CHUNKS;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     unsigned char* stage_w = smem;
@@ -139,12 +137,11 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     bool ok = true;
     if (warp == 0) {
         if (lane == 0) {
-            const int x_tiles = min(XTILES, (p.m - tok0 + TILE_ROWS - 1) / TILE_ROWS);
             auto load_w = [&](int kb, int s) {
                 const int held = min(CHUNKS, chunks - kb * CHUNKS);
                 // spread codes count as they are packed, half of the space they take
                 mbar_expect_tx(&full[s], T::STAGE_W / (ABITS == 8 ? 2 : 1) + T::STAGE_X);
-                mbar_expect_tx(&scales_full[s], (unsigned)(held * (1 + x_tiles) * TILE_BYTES));
+                mbar_expect_tx(&scales_full[s], (unsigned)(held * 2 * TILE_BYTES));
                 tma_load_2d(stage_w + s * T::STAGE_W, &map_w, &full[s], kb * ROW, n0);
                 bulk_load(stage_s + s * T::STAGE_S, p.w_scales + ((size_t)(n0 / TILE_ROWS) * chunks + kb * CHUNKS) * TILE_BYTES,
                           (unsigned)(held * TILE_BYTES), smem_u32(&scales_full[s]));
@@ -162,10 +159,9 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 }
                 const int held = min(CHUNKS, chunks - kb * CHUNKS);
                 tma_load_2d(stage_x + s * T::STAGE_X, &map_x, &full[s], kb * ROW, tok0);
-                for (int j = 0; j < x_tiles; ++j)
-                    bulk_load(stage_s + s * T::STAGE_S + CHUNKS * (1 + j) * TILE_BYTES,
-                              p.x_scales + ((size_t)(tok0 / TILE_ROWS + j) * chunks + kb * CHUNKS) * TILE_BYTES,
-                              (unsigned)(held * TILE_BYTES), smem_u32(&scales_full[s]));
+                bulk_load(stage_s + s * T::STAGE_S + CHUNKS * TILE_BYTES,
+                          p.x_scales + ((size_t)(tok0 / TILE_ROWS) * chunks + kb * CHUNKS) * TILE_BYTES,
+                          (unsigned)(held * TILE_BYTES), smem_u32(&scales_full[s]));
             }
         }
     } else if (warp == 1) {
@@ -183,7 +179,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 for (int kk = 0; kk < 4; ++kk) {              // 32 bytes of every row: 64 or 32 elements
                     const int j = ABITS == 4 ? kk / 2 : 0;
                     if (j >= held) break;
-                    const unsigned sf = cols + j * 4 * (1 + XTILES);
+                    const unsigned sf = cols + j * 8;
                     umma_scaled<ABITS>(tmem_base, dw + kk * 2, dx + kk * 2, with_ids(idesc, ABITS == 4 ? kk % 2 * 2 : kk), sf,
                                        sf + 4, it > 0 || kk > 0);
                 }
@@ -194,7 +190,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     } else {
         const int quarter = warp & 3, row = quarter * 32 + lane;
         const unsigned acc = tmem_base + ((unsigned)(quarter * 32) << 16);
-        // a stage's scale tiles into the stage's columns: W's four, then four per tile of A, per chunk
+        // a stage's scale tiles into the stage's columns: W's four, then A's four, per chunk
         for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
             const int s = it % STAGES, held = min(CHUNKS, chunks - kb * CHUNKS);
             ok = __all_sync(0xffffffffu, mbar_wait(&scales_full[s], (it / STAGES) & 1));
@@ -202,8 +198,8 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             const uint4* from = reinterpret_cast<const uint4*>(stage_s + s * T::STAGE_S) + lane;
             for (int j = 0; j < held; ++j)
 #pragma unroll
-                for (int t = 0; t <= XTILES; ++t)
-                    tmem_store4(acc + T::ACC_COLS + s * T::SCALE_COLS + (j * (1 + XTILES) + t) * 4, from[(t * CHUNKS + j) * 32]);
+                for (int t = 0; t < 2; ++t)
+                    tmem_store4(acc + T::ACC_COLS + s * T::SCALE_COLS + j * 8 + t * 4, from[(t * CHUNKS + j) * 32]);
             tmem_stores_done();
             tc_fence_before();
             __syncwarp();
@@ -339,8 +335,7 @@ int launch(const void* w, const void* x, Args p, void* stream) {
 
 template <int ABITS, int OBITS> int launch_rows(const void* w, const void* x, const Args& p, void* stream) {
     return p.m <= 16 ? launch<16, ABITS, OBITS>(w, x, p, stream) : p.m <= 32 ? launch<32, ABITS, OBITS>(w, x, p, stream)
-         : p.m <= 64 ? launch<64, ABITS, OBITS>(w, x, p, stream) : p.m <= 128 ? launch<128, ABITS, OBITS>(w, x, p, stream)
-         : launch<256, ABITS, OBITS>(w, x, p, stream);
+         : p.m <= 64 ? launch<64, ABITS, OBITS>(w, x, p, stream) : launch<128, ABITS, OBITS>(w, x, p, stream);
 }
 
 bool use_pairs(int m, int n) { return m > 256; }

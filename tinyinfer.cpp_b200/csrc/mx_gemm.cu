@@ -338,7 +338,14 @@ template <int ABITS, int OBITS> int launch_rows(const void* w, const void* x, co
          : p.m <= 64 ? launch<64, ABITS, OBITS>(w, x, p, stream) : launch<128, ABITS, OBITS>(w, x, p, stream);
 }
 
-bool use_pairs(int m, int n) { return m > 256; }
+// Whether a product runs on pairs of SMs (mx_gemm_pairs.cu): with tiles of 256 x 256 for most of the 74 pairs, or where K is
+// too short to be cut.  Blocks of one SM win where their parts of K fill the GPU.  us, one SM / pairs: 512 x 4,096 x 12,288
+// (32 tiles) 30.9 / 39.1, 768 rows (48) 46.8 / 41.0, 512 x 6,144 x 4,096 (48) 19.3 / 18.0, 256 x 1,024 x 4,096 (4) 8.6 / 10.4,
+// 256 x 2,048 x 1,024 (8) 9.7 / 7.4, 1,024 x 2,048 x 512 (32) 9.9 / 6.5.  The gated form of one SM finishes many rows more
+// slowly: 128 x 2 x 12,288 x 4,096 27.3 / 18.5, 64 rows 23.4 / 27.8, 128 x 2 x 4,096 x 4,096 (32) 13.7 / 15.6.
+bool use_pairs(int m, int n, int kp, int from) {
+    return m > from && ((m + 255) / 256 * ((n + 255) / 256) >= 40 || kp <= 1024);
+}
 
 int check(const char* who, const void* a, const void* a_scales, int a_bits, const void* w, const void* w_scales, int m, int n,
           int kp) {
@@ -357,7 +364,7 @@ extern "C" int ti_mx_gemm(const void* a, const void* a_scales, int a_bits, const
     if (int rc = check("mx_gemm", a, a_scales, a_bits, w, w_scales, m, n, kp)) return rc;
     TI_REQUIRE((uintptr_t)c % 4 == 0 && ldc >= n, "mx_gemm: rows of %d floats for %d columns", ldc, n);
     if (m == 0 || n == 0) return 0;
-    if (use_pairs(m, n))
+    if (use_pairs(m, n, kp, 128))
         return mx_gemm_pairs(a, a_scales, a_bits, w, w_scales, c, m, n, kp, ldc, accumulate, settled, status, stream);
     const Args p{(const unsigned char*)w_scales, (const unsigned char*)a_scales, c, nullptr, nullptr, m, n, kp, ldc, 0,
                  accumulate ? MODE_ACCUMULATE : MODE_STORE, 1, 0, settled, status};
@@ -371,8 +378,9 @@ extern "C" int ti_mx_gemm_glu(const void* a, const void* a_scales, int a_bits, c
     TI_REQUIRE(out_bits == 4 || out_bits == 8, "mx_gemm_glu: output of %d bits (4 and 8 are known)", out_bits);
     TI_REQUIRE(out_kp % CHUNK == 0, "mx_gemm_glu: %d output columns are not whole chunks of 128", out_kp);
     if (m == 0 || out_kp == 0) return 0;
-    if (use_pairs(m, 2 * out_kp))
-        return mx_gemm_pairs_glu(a, a_scales, a_bits, w, w_scales, codes, scales, out_bits, m, out_kp, kp, settled, status, stream);
+    if (use_pairs(m, 2 * out_kp, kp, 64))
+        return mx_gemm_pairs_glu(a, a_scales, a_bits, w, w_scales, codes, scales, out_bits, m, out_kp, kp, settled, status,
+                                 stream);
     const Args p{(const unsigned char*)w_scales, (const unsigned char*)a_scales, nullptr, (unsigned char*)codes,
                  (unsigned char*)scales, m, 2 * out_kp, kp, 0, out_kp, MODE_GLU, 1, 0, settled, status};
     if (out_bits == 8) return a_bits == 4 ? launch_rows<4, 8>(w, a, p, stream) : launch_rows<8, 8>(w, a, p, stream);

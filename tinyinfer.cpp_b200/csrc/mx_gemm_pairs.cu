@@ -170,47 +170,32 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
     // bytes of spills without the exchange: 53.0 -> 49.8 us at 4,096 x 6,144 x 4,096).  2 x 72 + 2 x 184 = 4 x 128.
     if (warp < 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
-        if (warp == 0) {
+        if (warp == 0 || warp == 2 || warp == 3) {
+            // Three threads ask for a stage's data, since a thread needs some 80 cycles for every load: the M side's rows, the
+            // N side's, the scales.  W may be older than the kernel in front of this one; what else is read is not.
             if (lane == 0) {
-                    const unsigned full0 = map_to_rank(smem_u32(full), 0);    // the leader's barriers
-                auto expect = [&](int s) {
-                    if (rank == 0) mbar_expect_tx(&full[s], T::STAGE_BYTES);
-                    mbar_expect_tx(&scales_full[s], 3 * T::SCALES);
-                };
-                auto load_p = [&](int row, int kb, int s) {       // the block's own rows
-                    tma_load_pair(stage_p + s * T::SIDE, &map_p, full0 + 8 * s, kb * ROW, row);
-                    tma_load_2d(stage_s + s * 3 * T::SCALES, &map_ps, &scales_full[s], kb * (T::SCALES / 4), row / TILE_ROWS);
-                };
-                auto load_q = [&](int row, int kb, int s) {       // half of the tile's rows, the scales of all
-                    tma_load_pair(stage_q + s * T::SIDE, &map_q, full0 + 8 * s, kb * ROW, row + (int)rank * 128);
-                    unsigned char* at = stage_s + (s * 3 + 1) * T::SCALES;
-                    for (int t = 0; t < 2; ++t)
-                        tma_load_2d(at + t * T::SCALES, &map_qs, &scales_full[s], kb * (T::SCALES / 4), row / TILE_ROWS + t);
-                };
-                int primed = 0;
-                if (p.settled)                           // W is older than the kernel in front of this one
-                    for (int tile = pair; tile < num_tiles && primed < STAGES; tile += num_pairs) {
-                        const int w0 = tile / tiles_a * 256;
-                        for (int kb = 0; kb < num_kb && primed < STAGES; ++kb, ++primed) {
-                            expect(primed);
-                            if (GLU) load_q(w0, kb, primed);
-                            else load_p(w0 + (int)rank * 128, kb, primed);
-                        }
-                    }
-                pdl_wait();
-                int s = 0, it = 0;
+                const unsigned full0 = map_to_rank(smem_u32(full), 0);    // the leader's barriers
+                if (!(p.settled && warp == (GLU ? 2 : 0))) pdl_wait();
+                int s = 0;
                 unsigned phase = 1;                      // of "empty"
                 for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
                     const int a0 = tile % tiles_a * 256, w0 = tile / tiles_a * 256;
                     const int p0 = (GLU ? a0 : w0) + (int)rank * 128, q0 = GLU ? w0 : a0;
-                    for (int kb = 0; kb < num_kb; ++kb, ++it) {
-                        if (it >= primed) {
-                            ok = mbar_wait(&empty[s], phase);
-                            if (!ok) break;
-                            expect(s);
+                    for (int kb = 0; kb < num_kb; ++kb) {
+                        ok = mbar_wait(&empty[s], phase);
+                        if (!ok) break;
+                        if (warp == 0) {
+                            if (rank == 0) mbar_expect_tx(&full[s], T::STAGE_BYTES);      // of both blocks and both sides
+                            tma_load_pair(stage_p + s * T::SIDE, &map_p, full0 + 8 * s, kb * ROW, p0);
+                        } else if (warp == 2) {
+                            tma_load_pair(stage_q + s * T::SIDE, &map_q, full0 + 8 * s, kb * ROW, q0 + (int)rank * 128);
+                        } else {
+                            unsigned char* at = stage_s + s * 3 * T::SCALES;
+                            mbar_expect_tx(&scales_full[s], 3 * T::SCALES);
+                            tma_load_2d(at, &map_ps, &scales_full[s], kb * (T::SCALES / 4), p0 / TILE_ROWS);
+                            tma_load_2d(at + T::SCALES, &map_qs, &scales_full[s], kb * (T::SCALES / 4), q0 / TILE_ROWS);
+                            tma_load_2d(at + 2 * T::SCALES, &map_qs, &scales_full[s], kb * (T::SCALES / 4), q0 / TILE_ROWS + 1);
                         }
-                        if (!GLU || it >= primed) load_q(q0, kb, s);
-                        if (GLU || it >= primed) load_p(p0, kb, s);
                         if (++s == STAGES) s = 0, phase ^= 1;
                     }
                 }

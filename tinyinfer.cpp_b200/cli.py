@@ -14,7 +14,8 @@ The engine works on token ids.  A prompt is text if the model brings a tokenizer
 ``tokenizer.ggml.*`` metadata, a folder's ``tokenizer.json``; read by this package's own
 byte-level BPE tokenizer); otherwise, and always with ``--tokens``, it is a list of token ids
 separated by spaces or commas.  Added options: ``--tokens``, ``--dtype``, ``--chunk``,
-``--max-batched-tokens``, ``--max-num-seqs``, ``--page-size``, ``--kv-tokens``, and
+``--max-batched-tokens``, ``--max-num-seqs``, ``--page-size``, ``--kv-tokens``, ``--weights mxfp4`` (the
+layers' matrices in 4 bits, quantised when they are loaded), and
 ``--random-weights CONFIG.json`` to run a configuration with seeded random weights.
 """
 from __future__ import annotations
@@ -54,6 +55,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--max-num-seqs", type=int, default=16)
     ap.add_argument("--page-size", type=int, default=64)
     ap.add_argument("--kv-tokens", type=int, default=None, help="tokens the cache pool holds")
+    ap.add_argument("--weights", choices=["mxfp4"], default=None, help="hold the layers' matrices in this format")
     ap.add_argument("--random-weights", metavar="CONFIG.json",
                     help="run this configuration with random weights drawn from --seed")
     return ap
@@ -102,7 +104,7 @@ def main(argv=None) -> int:
 
     kwargs = dict(dtype=args.dtype, max_seq=args.max_seq, max_num_seqs=args.max_num_seqs,
                   max_batched_tokens=args.max_batched_tokens, chunk=args.chunk,
-                  page_size=args.page_size, kv_tokens=args.kv_tokens, cuda_graph=args.cuda_graph)
+                  page_size=args.page_size, kv_tokens=args.kv_tokens, cuda_graph=args.cuda_graph, weights=args.weights)
     if args.random_weights:
         with open(args.random_weights, "r", encoding="utf-8") as fh:
             llm = LLM(config=json.load(fh), seed=args.seed, **kwargs)

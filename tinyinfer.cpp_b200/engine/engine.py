@@ -44,6 +44,8 @@ class Engine:
     dtype        ``bfloat16``: the kernels and precisions of serving (bfloat16 activations and
                  cache, float32 residual stream, norms, softmax); ``float32``: everything in
                  true 32-bit arithmetic.
+    weights      None: as stored; ``mxfp4``: the layers' matrices in the microscaled 4-bit format, quantised when they
+                 are loaded (bfloat16 engines; pre-norm layers of plain attention and SwiGLU).
     max_tokens   how many tokens the cache holds over all live requests (each request's
                  count rounded up to whole pages); or ``num_pages`` directly.
     ops          the kernel set; by default the CUDA kernels, which must be available.
@@ -55,8 +57,10 @@ class Engine:
                  seed: Optional[int] = None, dtype="bfloat16", device="cuda:0",
                  page_size: int = 64, max_tokens: Optional[int] = None,
                  num_pages: Optional[int] = None, max_requests: int = 64, ops=None,
-                 step_graphs: bool = False):
+                 step_graphs: bool = False, weights: Optional[str] = None):
         self.dtype = parse_dtype(dtype)
+        if weights is not None and self.dtype != torch.bfloat16:
+            raise ValueError(f"weights={weights!r} needs a bfloat16 engine")
         self.device = torch.device(device)
         if ops is None:
             # a kernel set of its own: its switches and what it holds back belong to this engine
@@ -77,6 +81,9 @@ class Engine:
             raise ValueError("Engine needs a model folder, or a configuration and a seed")
         self.config = typed
         self.plan = arch.build_plan(typed)
+        if weights is not None:
+            from ..parts.microscaled import microscaled_plan
+            self.plan = microscaled_plan(self.plan, weights)
         self.model = CausalLM(self.plan)
         if gguf_file is not None:
             try:

@@ -51,19 +51,20 @@ class RunStats:
 class LLM:
     """model_dir or (config, seed); ``max_seq`` caps a request's context (the reference's
     ``--max-seq``, default 2048, src/main.cpp:131,150); the cache holds ``kv_tokens`` tokens
-    (default ``max_num_seqs * max_seq``, what the reference allocates, src/inference.cu:146-148)."""
+    (default ``max_num_seqs * max_seq``, what the reference allocates, src/inference.cu:146-148);
+    ``weights="mxfp4"`` keeps the layers' matrices in 4 bits (``Engine``)."""
 
     def __init__(self, model_dir: Optional[str] = None, *, config: Optional[Mapping[str, Any]] = None,
                  seed: Optional[int] = None, dtype="bfloat16", device="cuda:0",
                  max_seq: int = 2048, max_num_seqs: int = 16, max_batched_tokens: int = 2048,
                  chunk: Optional[int] = None, page_size: int = 64,
                  kv_tokens: Optional[int] = None, cuda_graph: bool = False, lookahead: bool = True,
-                 ops=None):
+                 ops=None, weights: Optional[str] = None):
         if kv_tokens is None:
             kv_tokens = max_num_seqs * max_seq
         self.engine = Engine(model_dir, config=config, seed=seed, dtype=dtype, device=device,
                              page_size=page_size, num_pages=-(-kv_tokens // page_size),
-                             max_requests=max_num_seqs, ops=ops, step_graphs=cuda_graph)
+                             max_requests=max_num_seqs, ops=ops, step_graphs=cuda_graph, weights=weights)
         self.max_seq = min(max_seq, self.engine.plan.max_position)
         self.max_num_seqs = max_num_seqs
         self.max_batched_tokens = max_batched_tokens

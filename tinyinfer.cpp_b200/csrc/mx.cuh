@@ -82,6 +82,13 @@ __device__ __forceinline__ unsigned map_to_rank(unsigned addr, unsigned rank) {
     return out;
 }
 
+// one lane of a whole warp, always the same
+__device__ __forceinline__ bool elect_one() {
+    unsigned mine;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(mine));
+    return mine != 0;
+}
+
 // ---- block-scaled products -----------------------------------------------------------------------
 
 // A scale tile goes into tensor memory as its bytes lie: lane l of each quarter gets bytes 16 l to 16 l + 15 in four columns.

@@ -111,7 +111,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     unsigned long long* acc_full = bars + 4 * STAGES;
     unsigned* tmem_slot = (unsigned*)(bars + 4 * STAGES + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int part = (int)cluster_rank(), unit = (int)blockIdx.x / p.parts;
     const int n0 = unit % p.tiles_n * BW, tok0 = unit / p.tiles_n * NTOK;
     const int chunks = p.kp / CHUNK, num_kb = (chunks + CHUNKS - 1) / CHUNKS;
@@ -135,58 +135,70 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     const unsigned tmem_base = *tmem_slot;
 
     bool ok = true;
+    // These two warps walk their loops as a whole and let one elected lane issue: what an instruction needs is then known to be
+    // the same for the warp (a loop of one lane alone pays for moving it there, some 80 cycles for every load).
     if (warp == 0) {
-        if (lane == 0) {
-            auto load_w = [&](int kb, int s) {
-                const int held = min(CHUNKS, chunks - kb * CHUNKS);
+        const bool issues = elect_one();
+        auto load_w = [&](int kb, int s) {
+            const int held = min(CHUNKS, chunks - kb * CHUNKS);
+            if (issues) {
                 // spread codes count as they are packed, half of the space they take
                 mbar_expect_tx(&full[s], T::STAGE_W / (ABITS == 8 ? 2 : 1) + T::STAGE_X);
                 mbar_expect_tx(&scales_full[s], (unsigned)(held * 2 * TILE_BYTES));
                 tma_load_2d(stage_w + s * T::STAGE_W, &map_w, &full[s], kb * ROW, n0);
                 bulk_load(stage_s + s * T::STAGE_S, p.w_scales + ((size_t)(n0 / TILE_ROWS) * chunks + kb * CHUNKS) * TILE_BYTES,
                           (unsigned)(held * TILE_BYTES), smem_u32(&scales_full[s]));
-            };
-            int primed = 0;
-            if (p.settled)                                    // W is older than the kernel in front of this one
-                for (; primed < STAGES && kb0 + primed < kb1; ++primed) load_w(kb0 + primed, primed);
-            pdl_wait();
-            for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
-                const int s = it % STAGES;
-                if (it >= primed) {
-                    ok = mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1);
-                    if (!ok) break;
-                    load_w(kb, s);
-                }
-                const int held = min(CHUNKS, chunks - kb * CHUNKS);
+            }
+        };
+        int primed = 0;
+        if (p.settled)                                        // W is older than the kernel in front of this one
+            for (; primed < STAGES && kb0 + primed < kb1; ++primed) load_w(kb0 + primed, primed);
+        pdl_wait();
+        int s = 0;
+        unsigned phase = 1;                                   // of "empty"
+        for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
+            if (it >= primed) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], phase));
+                if (!ok) break;
+                load_w(kb, s);
+            }
+            if (issues) {
                 tma_load_2d(stage_x + s * T::STAGE_X, &map_x, &full[s], kb * ROW, tok0);
                 bulk_load(stage_s + s * T::STAGE_S + CHUNKS * TILE_BYTES,
                           p.x_scales + ((size_t)(tok0 / TILE_ROWS) * chunks + kb * CHUNKS) * TILE_BYTES,
-                          (unsigned)(held * TILE_BYTES), smem_u32(&scales_full[s]));
+                          (unsigned)(min(CHUNKS, chunks - kb * CHUNKS) * TILE_BYTES), smem_u32(&scales_full[s]));
             }
+            if (++s == STAGES) s = 0, phase ^= 1;
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const unsigned idesc = ABITS == 4 ? scaled_idesc(BW, NTOK, FOUR_E2M1, FOUR_E2M1)
-                                              : scaled_idesc(BW, NTOK, MIXED_E2M1, MIXED_E4M3);
-            for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
-                const int s = it % STAGES, held = min(CHUNKS, chunks - kb * CHUNKS);
-                ok = mbar_wait(&full[s], (it / STAGES) & 1) && mbar_wait(&scaled[s], (it / STAGES) & 1);
-                if (!ok) break;
-                tc_fence_after();
-                const unsigned cols = tmem_base + T::ACC_COLS + s * T::SCALE_COLS;
-                const unsigned long long dw = umma_desc(stage_w + s * T::STAGE_W), dx = umma_desc(stage_x + s * T::STAGE_X);
+        const bool issues = elect_one();
+        const unsigned idesc = ABITS == 4 ? scaled_idesc(BW, NTOK, FOUR_E2M1, FOUR_E2M1)
+                                          : scaled_idesc(BW, NTOK, MIXED_E2M1, MIXED_E4M3);
+        int s = 0;
+        unsigned phase = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            const int held = min(CHUNKS, chunks - kb * CHUNKS);
+            ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase) && mbar_wait(&scaled[s], phase));
+            if (!ok) break;
+            tc_fence_after();
+            const unsigned cols = tmem_base + T::ACC_COLS + s * T::SCALE_COLS;
+            const unsigned long long dw = umma_desc(stage_w + s * T::STAGE_W), dx = umma_desc(stage_x + s * T::STAGE_X);
+            if (issues) {
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {              // 32 bytes of every row: 64 or 32 elements
                     const int j = ABITS == 4 ? kk / 2 : 0;
                     if (j >= held) break;
                     const unsigned sf = cols + j * 8;
                     umma_scaled<ABITS>(tmem_base, dw + kk * 2, dx + kk * 2, with_ids(idesc, ABITS == 4 ? kk % 2 * 2 : kk), sf,
-                                       sf + 4, it > 0 || kk > 0);
+                                       sf + 4, kb > kb0 || kk > 0);
                 }
                 umma_commit(&empty[s]);
             }
-            umma_commit(acc_full);
+            __syncwarp();
+            if (++s == STAGES) s = 0, phase ^= 1;
         }
+        if (issues) umma_commit(acc_full);
+        __syncwarp();
     } else {
         const int quarter = warp & 3, row = quarter * 32 + lane;
         const unsigned acc = tmem_base + ((unsigned)(quarter * 32) << 16);
@@ -314,8 +326,10 @@ int launch(const void* w, const void* x, Args p, void* stream) {
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     p.tiles_n = (p.n + BW - 1) / BW;
     const int tiles = p.tiles_n * ((p.m + NTOK - 1) / NTOK), num_kb = (p.kp + T::ELEMS - 1) / T::ELEMS;
+    // K in as many parts as find blocks at once (two an SM), in 8 only where a part is long enough to be worth the larger
+    // cluster: us with 4 / 8 parts, 8 rows x 4,096 x 4,096 (32 stages) 4.9 / 5.8, 8 x 4,096 x 12,288 (96) 9.0 / 7.9
     p.parts = 1;
-    while (p.parts < 8 && tiles * p.parts * 2 <= sms * T::PER_SM && p.parts * 2 <= num_kb) p.parts *= 2;
+    while (p.parts < (num_kb >= 40 ? 8 : 4) && tiles * p.parts * 2 <= sms * T::PER_SM && p.parts * 2 <= num_kb) p.parts *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = (unsigned)(tiles * p.parts);
     cfg.blockDim = THREADS;

@@ -136,7 +136,7 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
     unsigned long long *acc_full = bars + 4 * STAGES, *acc_empty = bars + 4 * STAGES + 1;    // in both; in the leader only
     unsigned* tmem_slot = (unsigned*)(bars + 4 * STAGES + 2);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const unsigned rank = cluster_rank();
     const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
     const int chunks = p.kp / CHUNK, num_kb = (chunks + CHUNKS - 1) / CHUNKS;
@@ -170,20 +170,21 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
     // bytes of spills without the exchange: 53.0 -> 49.8 us at 4,096 x 6,144 x 4,096).  2 x 72 + 2 x 184 = 4 x 128.
     if (warp < 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        // The warps below walk their loops as a whole and let one elected lane issue, as in mx_gemm.cu.  Three ask for a stage's
+        // data: the M side's rows, the N side's, the scales.
+        const bool issues = elect_one();
         if (warp == 0 || warp == 2 || warp == 3) {
-            // Three threads ask for a stage's data, since a thread needs some 80 cycles for every load: the M side's rows, the
-            // N side's, the scales.  W may be older than the kernel in front of this one; what else is read is not.
-            if (lane == 0) {
-                const unsigned full0 = map_to_rank(smem_u32(full), 0);    // the leader's barriers
-                if (!(p.settled && warp == (GLU ? 2 : 0))) pdl_wait();
-                int s = 0;
-                unsigned phase = 1;                      // of "empty"
-                for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
-                    const int a0 = tile % tiles_a * 256, w0 = tile / tiles_a * 256;
-                    const int p0 = (GLU ? a0 : w0) + (int)rank * 128, q0 = GLU ? w0 : a0;
-                    for (int kb = 0; kb < num_kb; ++kb) {
-                        ok = mbar_wait(&empty[s], phase);
-                        if (!ok) break;
+            const unsigned full0 = map_to_rank(smem_u32(full), 0);        // the leader's barriers
+            if (!(p.settled && warp == (GLU ? 2 : 0))) pdl_wait();        // W may be older than the kernel in front of this one
+            int s = 0;
+            unsigned phase = 1;                          // of "empty"
+            for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+                const int a0 = tile % tiles_a * 256, w0 = tile / tiles_a * 256;
+                const int p0 = (GLU ? a0 : w0) + (int)rank * 128, q0 = GLU ? w0 : a0;
+                for (int kb = 0; kb < num_kb; ++kb) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], phase));
+                    if (!ok) break;
+                    if (issues) {
                         if (warp == 0) {
                             if (rank == 0) mbar_expect_tx(&full[s], T::STAGE_BYTES);      // of both blocks and both sides
                             tma_load_pair(stage_p + s * T::SIDE, &map_p, full0 + 8 * s, kb * ROW, p0);
@@ -196,38 +197,43 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
                             tma_load_2d(at + T::SCALES, &map_qs, &scales_full[s], kb * (T::SCALES / 4), q0 / TILE_ROWS);
                             tma_load_2d(at + 2 * T::SCALES, &map_qs, &scales_full[s], kb * (T::SCALES / 4), q0 / TILE_ROWS + 1);
                         }
-                        if (++s == STAGES) s = 0, phase ^= 1;
                     }
+                    if (++s == STAGES) s = 0, phase ^= 1;
                 }
             }
         } else if (warp == 1) {
-            if (rank == 0 && lane == 0) {
+            if (rank == 0) {
                 const unsigned idesc = ABITS == 4 ? scaled_idesc(BM, BN, FOUR_E2M1, FOUR_E2M1)
                                      : GLU ? scaled_idesc(BM, BN, MIXED_E4M3, MIXED_E2M1) : scaled_idesc(BM, BN, MIXED_E2M1, MIXED_E4M3);
                 int s = 0, local = 0;
                 unsigned phase = 0;
                 for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local) {
-                    ok = mbar_wait(acc_empty, (local & 1) ^ 1);
+                    ok = __all_sync(0xffffffffu, mbar_wait(acc_empty, (local & 1) ^ 1));
                     if (!ok) break;
                     tc_fence_after();
                     for (int kb = 0; kb < num_kb; ++kb) {
                         const int held = min(CHUNKS, chunks - kb * CHUNKS);
-                        ok = mbar_wait(&full[s], phase) && mbar_wait(&scaled[s], phase);
+                        ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase) && mbar_wait(&scaled[s], phase));
                         if (!ok) break;
                         tc_fence_after();
                         const unsigned cols = tmem_base + BN + s * T::SCALE_COLS;
                         const unsigned long long da = umma_desc(stage_p + s * T::SIDE), db = umma_desc(stage_q + s * T::SIDE);
+                        if (issues) {
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) {
-                            const int j = ABITS == 4 ? kk / 2 : 0;
-                            if (j >= held) break;
-                            umma_scaled_pair<ABITS>(tmem_base, da + kk * 2, db + kk * 2, with_ids(idesc, ABITS == 4 ? kk % 2 * 2 : kk),
-                                                    cols + j * 12, cols + j * 12 + 4, (kb | kk) != 0);
+                            for (int kk = 0; kk < 4; ++kk) {
+                                const int j = ABITS == 4 ? kk / 2 : 0;
+                                if (j >= held) break;
+                                umma_scaled_pair<ABITS>(tmem_base, da + kk * 2, db + kk * 2,
+                                                        with_ids(idesc, ABITS == 4 ? kk % 2 * 2 : kk), cols + j * 12,
+                                                        cols + j * 12 + 4, (kb | kk) != 0);
+                            }
+                            commit_pair(&empty[s]);
                         }
-                        commit_pair(&empty[s]);
+                        __syncwarp();
                         if (++s == STAGES) s = 0, phase ^= 1;
                     }
-                    commit_pair(acc_full);
+                    if (issues) commit_pair(acc_full);
+                    __syncwarp();
                 }
             }
         } else if (warp >= 4) {

@@ -285,16 +285,17 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
                     float* dst = p.c + (size_t)tok * p.ldc + n0 + mine;
 #pragma unroll
                     for (int t0 = 0; t0 < 128; t0 += 32) {
+                        const float* from = dst;                    // the address steps on: 128 of them do not fit the registers
                         if (p.accumulate) {                         // old values are asked for 32 at a time
                             float old[32];
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) old[i] = t0 + i < held ? __ldcg(dst + (size_t)(t0 + i) * p.ldc) : 0.0f;
+                            for (int i = 0; i < 32; ++i, from += p.ldc) old[i] = t0 + i < held ? __ldcg(from) : 0.0f;
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[t0 + i] = __float_as_uint(old[i] + __uint_as_float(v[t0 + i]));
                         }
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (t0 + i < held) dst[(size_t)(t0 + i) * p.ldc] = __uint_as_float(v[t0 + i]);
+                        for (int i = 0; i < 32; ++i, dst += p.ldc)
+                            if (t0 + i < held) *dst = __uint_as_float(v[t0 + i]);
                     }
                 }
             }

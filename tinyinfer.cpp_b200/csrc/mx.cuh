@@ -65,6 +65,14 @@ __device__ __forceinline__ unsigned codes_e2m1x8(const float* y) {
     return r;
 }
 
+// g / (1 + e^-g) with the approximate exponential and reciprocal (about 1e-6 of the result, far below the rounding to 8 bits);
+// -0 for very negative g
+__device__ __forceinline__ float silu(float g) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-g)));
+    return g * r;
+}
+
 // ---- clusters ------------------------------------------------------------------------------------
 
 __device__ __forceinline__ unsigned cluster_rank() {

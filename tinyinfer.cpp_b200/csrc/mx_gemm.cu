@@ -81,7 +81,7 @@ __device__ __forceinline__ void umma_scaled(unsigned tmem_d, unsigned long long 
 // The gated rows of a token's 64 outputs of this tile, summed over the parts, as codes: lanes are the 32 outputs of a block.
 template <int OBITS>
 __device__ __forceinline__ void finish_glu(const Args& p, float gate, float up, int tok, int out_col, int lane) {
-    const float h = up * gate / (1.0f + expf(-gate));
+    const float h = silu(gate) * up;
     const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
     const unsigned s = scale_byte<OBITS>(top);
     const float y = h * scale_inverse(s);

@@ -101,7 +101,7 @@ __device__ __forceinline__ void finish_glu(const Args& p, const unsigned* gate, 
     unsigned top = 0;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-        h[i] = silu_mul(__uint_as_float(gate[i]), __uint_as_float(up[i]));
+        h[i] = silu(__uint_as_float(gate[i])) * __uint_as_float(up[i]);
         top = max(top, __float_as_uint(h[i]) & 0x7fffffffu);
     }
     const unsigned s = scale_byte<OBITS>(top);

@@ -99,16 +99,14 @@ __device__ __forceinline__ bool elect_one() {
 
 // ---- block-scaled products -----------------------------------------------------------------------
 
-// A scale tile goes into tensor memory as its bytes lie: lane l of each quarter gets bytes 16 l to 16 l + 15 in four columns.
-// Threads store it (a tile is one 16-byte read of shared memory and one tcgen05.st per lane).  tcgen05.cp would do it without
-// threads, but runs in line with the products: 2.4 PFLOP/s of 4-bit products 0.17 us shorter per 256 of K without it, a
-// quarter of the time (4,096 x 6,144 x 4,096 65.1 -> 49.8 us, 2,048 x 24,576 x 4,096 115.8 -> 85.9 us).
-__device__ __forceinline__ void tmem_store4(unsigned taddr, const uint4& v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};\n"
-                 ::"r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+// A scale tile as tcgen05.cp reads it: 32 rows of 16 bytes without a swizzle, groups of 8 rows 128 bytes apart.  The copies run
+// in line with the products.  They and the products have to be issued by an elected lane of a warp that walks its loop as a
+// whole: from a loop of one lane alone the same copies cost a quarter of the time of 4-bit products (4,096 x 6,144 x 4,096 65.1
+// against 49.8 us with the scales stored by other warps, which elected issue makes no faster than the copies).
+__device__ __forceinline__ unsigned long long scale_desc(const void* p) {
+    return (unsigned long long)((sm100::smem_u32(p) & 0x3FFFF) >> 4) | (unsigned long long)1 << 16 |
+           (unsigned long long)(128 >> 4) << 32 | (unsigned long long)1 << 46;
 }
-__device__ __forceinline__ void tmem_stores_done() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
-
 // Instruction descriptor of a block-scaled product with power-of-two scales; the scale bytes of a step of K are chosen in
 // their 32-bit words by `id` (bits 4-5 for B, 29-30 for A).
 __device__ __forceinline__ unsigned scaled_idesc(int m, int n, unsigned a_type, unsigned b_type) {

@@ -4,13 +4,16 @@
 // The roles of the operands are swapped: 128 rows of W are the instruction's M side, NTOK rows of A its N side, so a step of
 // few rows streams W once and wastes nothing on empty rows of A.  A stage of the ring is 128 bytes of every operand row: 256
 // elements where both sides have 4 bits, 128 where A has 8 (W's codes then take a byte each in shared memory; the spreading
-// is TMA's), with the scale tiles of those elements beside it.  The epilogue warps, idle until the sums are there, store a
-// stage's scale tiles into tensor memory columns of that stage (mx.cuh says why not tcgen05.cp); columns are written again
-// when the stage's "empty" barrier has seen the products that read them.
+// is TMA's), with the scale tiles of those elements beside it.  The MMA warp copies a stage's scale tiles into tensor memory
+// columns of that stage; columns are written again when the stage's "empty" barrier has seen the products that read them.
+//
+// Bound by TMA: a block takes 0.25 us a stage whether it has 5 stages in flight or 11, with 8 KB of 4-bit weights in a stage
+// that spreads them and 16 KB in one that does not, so one request's 151,936 x 4,096 runs at 5.4 and 5.9 TB/s; for few tiles by
+// the latency of a stage and of the launch (1 x 1,024 x 1,024 3.0 us).
 //
 // K is cut over the blocks of a cluster: each keeps its part of the sum in its shared memory, and after a cluster barrier
 // every block adds the parts of its share of the tokens, in the order of the blocks (no atomics: the same bits each run).
-// The number of parts depends on N, K and the tile alone.
+// The number of parts depends on the sizes alone.
 //
 // W's rows for the gated form are strips of 32 gate rows and their 32 up rows: 32 outputs are one warp's lanes and one block
 // of the format.
@@ -32,8 +35,10 @@ template <int NTOK, int ABITS> struct Tile {
     static constexpr int ELEMS = ABITS == 4 ? 256 : 128;                 // of K in a stage
     static constexpr int CHUNKS = ELEMS / CHUNK;
     static constexpr int STAGE_W = BW * ROW, STAGE_X = NTOK * ROW, STAGE_S = CHUNKS * 2 * TILE_BYTES;
-    static constexpr int PER_SM = 2;                                      // blocks of an SM
-    static constexpr int STAGES = NTOK == 128 ? 3 : NTOK == 64 ? 4 : 5;
+    // blocks of an SM, stages of a block's ring: two short rings for few rows (8 x 4,096 x 12,288 7.7 us, one of 11 stages 9.3),
+    // one long one where a stage is large (128 x 4,096 x 12,288 14.7 us with two of three stages, 12.9 with one of six)
+    static constexpr int PER_SM = NTOK == 128 ? 1 : 2;
+    static constexpr int STAGES = NTOK == 128 ? 6 : NTOK == 64 ? 4 : 5;
     static constexpr int SMEM = STAGES * (STAGE_W + STAGE_X + STAGE_S) + 1024 + 256;
     static constexpr int SCALE_COLS = CHUNKS * 8;                         // tensor memory columns of a stage's scales
     static constexpr int ACC_COLS = NTOK < 32 ? 32 : NTOK;
@@ -62,6 +67,9 @@ __device__ __forceinline__ float4 load_cluster4(unsigned addr) {
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
+}
+__device__ __forceinline__ void copy_scales(unsigned tmem, const void* tile) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(scale_desc(tile)) : "memory");
 }
 template <int ABITS>
 __device__ __forceinline__ void umma_scaled(unsigned tmem_d, unsigned long long da, unsigned long long db, unsigned idesc,
@@ -107,9 +115,8 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     unsigned char* stage_s = smem + STAGES * (T::STAGE_W + T::STAGE_X);
     unsigned long long* bars = (unsigned long long*)(stage_s + STAGES * T::STAGE_S);
     unsigned long long *full = bars, *empty = bars + STAGES;             // operands: TMA -> MMA, MMA -> TMA
-    unsigned long long *scales_full = bars + 2 * STAGES, *scaled = bars + 3 * STAGES;     // scales: TMA -> epilogue warps -> MMA
-    unsigned long long* acc_full = bars + 4 * STAGES;
-    unsigned* tmem_slot = (unsigned*)(bars + 4 * STAGES + 1);
+    unsigned long long* acc_full = bars + 2 * STAGES;
+    unsigned* tmem_slot = (unsigned*)(bars + 2 * STAGES + 1);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int part = (int)cluster_rank(), unit = (int)blockIdx.x / p.parts;
@@ -121,8 +128,6 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
-            mbar_init(&scales_full[s], 1);
-            mbar_init(&scaled[s], 4);
         }
         mbar_init(acc_full, 1);
         mbar_fence_init();
@@ -143,11 +148,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             const int held = min(CHUNKS, chunks - kb * CHUNKS);
             if (issues) {
                 // spread codes count as they are packed, half of the space they take
-                mbar_expect_tx(&full[s], T::STAGE_W / (ABITS == 8 ? 2 : 1) + T::STAGE_X);
-                mbar_expect_tx(&scales_full[s], (unsigned)(held * 2 * TILE_BYTES));
+                mbar_expect_tx(&full[s], (unsigned)(T::STAGE_W / (ABITS == 8 ? 2 : 1) + T::STAGE_X + held * 2 * TILE_BYTES));
                 tma_load_2d(stage_w + s * T::STAGE_W, &map_w, &full[s], kb * ROW, n0);
                 bulk_load(stage_s + s * T::STAGE_S, p.w_scales + ((size_t)(n0 / TILE_ROWS) * chunks + kb * CHUNKS) * TILE_BYTES,
-                          (unsigned)(held * TILE_BYTES), smem_u32(&scales_full[s]));
+                          (unsigned)(held * TILE_BYTES), smem_u32(&full[s]));
             }
         };
         int primed = 0;
@@ -166,7 +170,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 tma_load_2d(stage_x + s * T::STAGE_X, &map_x, &full[s], kb * ROW, tok0);
                 bulk_load(stage_s + s * T::STAGE_S + CHUNKS * TILE_BYTES,
                           p.x_scales + ((size_t)(tok0 / TILE_ROWS) * chunks + kb * CHUNKS) * TILE_BYTES,
-                          (unsigned)(min(CHUNKS, chunks - kb * CHUNKS) * TILE_BYTES), smem_u32(&scales_full[s]));
+                          (unsigned)(min(CHUNKS, chunks - kb * CHUNKS) * TILE_BYTES), smem_u32(&full[s]));
             }
             if (++s == STAGES) s = 0, phase ^= 1;
         }
@@ -178,12 +182,19 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         unsigned phase = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
             const int held = min(CHUNKS, chunks - kb * CHUNKS);
-            ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase) && mbar_wait(&scaled[s], phase));
+            ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase));
             if (!ok) break;
             tc_fence_after();
             const unsigned cols = tmem_base + T::ACC_COLS + s * T::SCALE_COLS;
             const unsigned long long dw = umma_desc(stage_w + s * T::STAGE_W), dx = umma_desc(stage_x + s * T::STAGE_X);
             if (issues) {
+                const unsigned char* scales = stage_s + s * T::STAGE_S;
+#pragma unroll
+                for (int j = 0; j < CHUNKS; ++j) {            // columns of a chunk: W's four, then A's four
+                    if (j >= held) break;
+                    copy_scales(cols + j * 8, scales + j * TILE_BYTES);
+                    copy_scales(cols + j * 8 + 4, scales + (CHUNKS + j) * TILE_BYTES);
+                }
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {              // 32 bytes of every row: 64 or 32 elements
                     const int j = ABITS == 4 ? kk / 2 : 0;
@@ -202,21 +213,6 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     } else {
         const int quarter = warp & 3, row = quarter * 32 + lane;
         const unsigned acc = tmem_base + ((unsigned)(quarter * 32) << 16);
-        // a stage's scale tiles into the stage's columns: W's four, then A's four, per chunk
-        for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
-            const int s = it % STAGES, held = min(CHUNKS, chunks - kb * CHUNKS);
-            ok = __all_sync(0xffffffffu, mbar_wait(&scales_full[s], (it / STAGES) & 1));
-            if (!ok) break;
-            const uint4* from = reinterpret_cast<const uint4*>(stage_s + s * T::STAGE_S) + lane;
-            for (int j = 0; j < held; ++j)
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    tmem_store4(acc + T::ACC_COLS + s * T::SCALE_COLS + j * 8 + t * 4, from[(t * CHUNKS + j) * 32]);
-            tmem_stores_done();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&scaled[s]);
-        }
         pdl_wait();                                           // C belongs to the chain of launches
         ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_full, 0));
         tc_fence_after();

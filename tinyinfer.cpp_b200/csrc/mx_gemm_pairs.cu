@@ -3,16 +3,20 @@
 // Two blocks of a cluster compute one tile of 256 rows of A and 256 rows of W together; each fetches 128 rows of either, both
 // tensor cores read both blocks' N side.  A stage is 128 bytes of every operand row (256 elements where both sides have 4
 // bits, 128 where A has 8) and the scale tiles of those elements: the block's own rows' for the M side, all 256 rows' for the
-// N side.  Four warps of each block store a stage's scale tiles into its tensor memory, the leader's MMA thread issues the
-// products.
+// N side.  The leader's MMA warp copies a stage's scales into tensor memory columns of that stage (each SM from its own shared
+// memory) and issues the products.
 //
 // The gated form has A's rows on the M side: a thread then holds a row's 32 gates and their 32 ups, a block of the format.
 // The plain form has W's rows there: a warp's lanes are 32 neighbouring columns of C, whose stores and, when adding to C, loads
-// are whole lines (a row of C per lane instead, in stores of 32 bytes: XXX).
+// are whole lines (with a row of C a lane and 32 bytes an access, adding cost 15 us more at 2,048 x 4,096 x 12,288, now 6).
 //
 // Tensor memory holds one accumulator of 256 columns and the scales of every stage; there is no room for a second one.  So the
 // eight epilogue warps read a tile's sums into registers (128 a thread), hand the accumulator back, and store from registers
 // while the next tile's products run.
+//
+// Bound by the tensor cores and, in long runs, by the power limit: in a graph of 20 launches 2,048 x 24,576 x 4,096 gated takes
+// 74.6 us with 4-bit rows (5.5 PFLOP/s, tensor pipes busy in 71 % of the cycles) and 136 with 8-bit rows (3.0 PFLOP/s);
+// back to back for seconds a fifth more.
 //
 // Every wait is bounded; on a timeout the block records status 2 and both blocks leave through the cluster barrier.
 #include "mx.cuh"
@@ -22,7 +26,7 @@ namespace {
 using namespace sm100;
 using namespace mx;
 
-constexpr int BM = 256, BN = 256, THREADS = 512;        // warpgroups: TMA and MMA warps, scale warps, two of epilogue
+constexpr int BM = 256, BN = 256, THREADS = 384;        // TMA, MMA, TMA, TMA warps; two warpgroups of epilogue
 constexpr int ROW = 128;                                // bytes of an operand row in a stage
 enum { TI_ERR_TIMEOUT = 2 };
 
@@ -30,9 +34,9 @@ template <int ABITS> struct Pair {
     static constexpr int ELEMS = ABITS == 4 ? 256 : 128, CHUNKS = ELEMS / CHUNK;
     static constexpr int SIDE = 128 * ROW, SCALES = CHUNKS * TILE_BYTES;      // operand rows and scale tiles of a block
     static constexpr int STAGES = 6;
-    static constexpr int SMEM = STAGES * (2 * SIDE + 3 * SCALES) + 1024 + 512;
+    static constexpr int SMEM = STAGES * (2 * SIDE + 3 * SCALES) + 1024 + 256;
     // what TMA counts for a stage, both blocks: spread codes count as they are packed
-    static constexpr unsigned STAGE_BYTES = 2 * (SIDE + SIDE / (ABITS == 8 ? 2 : 1));
+    static constexpr unsigned STAGE_BYTES = 2 * (SIDE + SIDE / (ABITS == 8 ? 2 : 1) + 3 * SCALES);
     static constexpr int SCALE_COLS = CHUNKS * 12;       // the M side's four columns, the N side's eight, per chunk
     static_assert(BN + STAGES * SCALE_COLS <= 512, "tensor memory");
     static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -60,6 +64,9 @@ __device__ __forceinline__ void commit_pair(void* bar) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
         ::"r"(smem_u32(bar)), "h"(mask) : "memory");
+}
+__device__ __forceinline__ void copy_scales_pair(unsigned tmem, const void* tile) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(scale_desc(tile)) : "memory");
 }
 template <int ABITS>
 __device__ __forceinline__ void umma_scaled_pair(unsigned tmem_d, unsigned long long da, unsigned long long db, unsigned idesc,
@@ -131,10 +138,8 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
     unsigned long long* bars = (unsigned long long*)(stage_s + STAGES * 3 * T::SCALES);
     unsigned long long* full = bars;                     // [STAGES] used in the leader only
     unsigned long long* empty = bars + STAGES;           // [STAGES] in both blocks
-    unsigned long long* scales_full = bars + 2 * STAGES;  // [STAGES] in both blocks, each its own scales' bytes
-    unsigned long long* scaled = bars + 3 * STAGES;      // [STAGES] used in the leader only: scales are in tensor memory
-    unsigned long long *acc_full = bars + 4 * STAGES, *acc_empty = bars + 4 * STAGES + 1;    // in both; in the leader only
-    unsigned* tmem_slot = (unsigned*)(bars + 4 * STAGES + 2);
+    unsigned long long *acc_full = bars + 2 * STAGES, *acc_empty = bars + 2 * STAGES + 1;    // in both; in the leader only
+    unsigned* tmem_slot = (unsigned*)(bars + 2 * STAGES + 2);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const unsigned rank = cluster_rank();
@@ -146,8 +151,6 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
-            mbar_init(&scales_full[s], 1);
-            mbar_init(&scaled[s], 8);
         }
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 16);
@@ -166,14 +169,14 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
     const unsigned tmem_base = *tmem_slot;
 
     bool ok = true;
-    // Registers: the block starts with 128 a thread; an epilogue thread needs its 128 sums and what it stores them with (160
-    // bytes of spills without the exchange: 53.0 -> 49.8 us at 4,096 x 6,144 x 4,096).  2 x 72 + 2 x 184 = 4 x 128.
-    if (warp < 8) {
+    // Registers: the block starts with 168 a thread; an epilogue thread needs its 128 sums, 32 old values and what it stores
+    // them with.  72 + 2 x 216 = 3 x 168.
+    if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
         // The warps below walk their loops as a whole and let one elected lane issue, as in mx_gemm.cu.  Three ask for a stage's
         // data: the M side's rows, the N side's, the scales.
         const bool issues = elect_one();
-        if (warp == 0 || warp == 2 || warp == 3) {
+        if (warp != 1) {
             const unsigned full0 = map_to_rank(smem_u32(full), 0);        // the leader's barriers
             if (!(p.settled && warp == (GLU ? 2 : 0))) pdl_wait();        // W may be older than the kernel in front of this one
             int s = 0;
@@ -192,16 +195,15 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
                             tma_load_pair(stage_q + s * T::SIDE, &map_q, full0 + 8 * s, kb * ROW, q0 + (int)rank * 128);
                         } else {
                             unsigned char* at = stage_s + s * 3 * T::SCALES;
-                            mbar_expect_tx(&scales_full[s], 3 * T::SCALES);
-                            tma_load_2d(at, &map_ps, &scales_full[s], kb * (T::SCALES / 4), p0 / TILE_ROWS);
-                            tma_load_2d(at + T::SCALES, &map_qs, &scales_full[s], kb * (T::SCALES / 4), q0 / TILE_ROWS);
-                            tma_load_2d(at + 2 * T::SCALES, &map_qs, &scales_full[s], kb * (T::SCALES / 4), q0 / TILE_ROWS + 1);
+                            tma_load_pair(at, &map_ps, full0 + 8 * s, kb * (T::SCALES / 4), p0 / TILE_ROWS);
+                            tma_load_pair(at + T::SCALES, &map_qs, full0 + 8 * s, kb * (T::SCALES / 4), q0 / TILE_ROWS);
+                            tma_load_pair(at + 2 * T::SCALES, &map_qs, full0 + 8 * s, kb * (T::SCALES / 4), q0 / TILE_ROWS + 1);
                         }
                     }
                     if (++s == STAGES) s = 0, phase ^= 1;
                 }
             }
-        } else if (warp == 1) {
+        } else {
             if (rank == 0) {
                 const unsigned idesc = ABITS == 4 ? scaled_idesc(BM, BN, FOUR_E2M1, FOUR_E2M1)
                                      : GLU ? scaled_idesc(BM, BN, MIXED_E4M3, MIXED_E2M1) : scaled_idesc(BM, BN, MIXED_E2M1, MIXED_E4M3);
@@ -213,12 +215,20 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
                     tc_fence_after();
                     for (int kb = 0; kb < num_kb; ++kb) {
                         const int held = min(CHUNKS, chunks - kb * CHUNKS);
-                        ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase) && mbar_wait(&scaled[s], phase));
+                        ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase));
                         if (!ok) break;
                         tc_fence_after();
                         const unsigned cols = tmem_base + BN + s * T::SCALE_COLS;
                         const unsigned long long da = umma_desc(stage_p + s * T::SIDE), db = umma_desc(stage_q + s * T::SIDE);
+                        const unsigned char* scales = stage_s + s * 3 * T::SCALES;
                         if (issues) {
+#pragma unroll
+                            for (int j = 0; j < CHUNKS; ++j) {          // columns of a chunk: the M side's four, the N side's eight
+                                if (j >= held) break;
+#pragma unroll
+                                for (int t = 0; t < 3; ++t)
+                                    copy_scales_pair(cols + j * 12 + t * 4, scales + t * T::SCALES + j * TILE_BYTES);
+                            }
 #pragma unroll
                             for (int kk = 0; kk < 4; ++kk) {
                                 const int j = ABITS == 4 ? kk / 2 : 0;
@@ -236,28 +246,10 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
                     __syncwarp();
                 }
             }
-        } else if (warp >= 4) {
-            // A stage's scale tiles into the stage's columns of tensor memory, each warp its 32 lanes.
-            const unsigned acc = tmem_base + ((unsigned)((warp & 3) * 32) << 16) + BN;
-            const int mine = num_tiles > pair ? (num_tiles - pair + num_pairs - 1) / num_pairs : 0;
-            for (int it = 0; it < mine * num_kb; ++it) {
-                const int s = it % STAGES;
-                ok = __all_sync(0xffffffffu, mbar_wait(&scales_full[s], (it / STAGES) & 1));
-                if (!ok) break;
-                const uint4* from = reinterpret_cast<const uint4*>(stage_s + s * 3 * T::SCALES) + lane;
-#pragma unroll
-                for (int j = 0; j < CHUNKS; ++j)
-#pragma unroll
-                    for (int t = 0; t < 3; ++t) tmem_store4(acc + s * T::SCALE_COLS + j * 12 + t * 4, from[(t * CHUNKS + j) * 32]);
-                tmem_stores_done();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&scaled[s]), 0));
-            }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;\n");
-        const int quarter = warp & 3, half = (warp - 8) >> 2;       // the lanes this warp may read; half of the columns
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
+        const int quarter = warp & 3, half = (warp - 4) >> 2;       // the lanes this warp may read; half of the columns
         const unsigned acc = tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)(half * 128);
         pdl_wait();                                                 // the output belongs to the chain of launches
         int local = 0;

@@ -170,9 +170,9 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
 
     bool ok = true;
     // Registers: the block starts with 168 a thread; an epilogue thread needs its 128 sums, 32 old values and what it stores
-    // them with.  72 + 2 x 216 = 3 x 168.
+    // them with.  120 + 2 x 192 = 3 x 168.
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;\n");
         // The warps below walk their loops as a whole and let one elected lane issue, as in mx_gemm.cu.  Three ask for a stage's
         // data: the M side's rows, the N side's, the scales.
         const bool issues = elect_one();
@@ -248,7 +248,7 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;\n");
         const int quarter = warp & 3, half = (warp - 4) >> 2;       // the lanes this warp may read; half of the columns
         const unsigned acc = tmem_base + ((unsigned)(quarter * 32) << 16) + (unsigned)(half * 128);
         pdl_wait();                                                 // the output belongs to the chain of launches

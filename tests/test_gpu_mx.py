@@ -307,6 +307,21 @@ def test_on_a_stream_of_its_own_and_in_a_graph(ops):
     fine(ops)
 
 
+def test_held_back_products_run_first(ops):
+    """A product that another part let the kernel set hold back is in the residual before the norm reads it."""
+    from tinyinfer_b200.kernels import CudaOps
+    mine = CudaOps("cuda:0")
+    a, w = (torch.randn(s, device="cuda", generator=gen(i)).bfloat16() for i, s in enumerate(((4, 256), (512, 256))))
+    x, ones = torch.randn(4, 512, device="cuda", generator=gen(5)), torch.ones(512, device="cuda")
+    want = x.clone()
+    mine.linear(a, w, want, accumulate=True)
+    want = mine.mx_dequantize(mine.mx_rmsnorm(want, ones, 1e-6))
+    mine.linear(a, w, x, accumulate=True, may_defer=True)
+    assert mine._pending is not None
+    assert torch.equal(mine.mx_dequantize(mine.mx_rmsnorm(x, ones, 1e-6)), want)
+    assert mine._pending is None
+
+
 def test_no_rows(ops):
     w = ops.mx_pack_linear(torch.randn(8, 64, device="cuda"))
     q = ops.mx_quantize(torch.empty(0, 64, device="cuda"), 8)

@@ -3,11 +3,12 @@
 //
 // The other libraries are called through ctypes, where a call with its checks and two new outputs costs 9 to 15 us of host
 // time; the kernels behind these operators take 2 to 10 for few rows, so an eager step would wait for its host.  Here a call
-// costs about what its launch costs (us, through ctypes -> here: quantisation of 8 rows 12.7 -> 5.4, norm 14.6 -> 5.6, product
-// 9.3 -> 5.1).
+// costs about what its launch costs (us, through ctypes -> here: quantisation of 8 rows 12.7 -> 4.2, norm 14.6 -> 4.4, product
+// 9.3 -> 3.4).
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -51,6 +52,10 @@ int64_t number(PyObject* o, const char* who, const char* what) {
     if (PyErr_Occurred()) PyErr_Clear();
     need(PyLong_Check(o) && v >= -(1LL << 31) && v < (1LL << 31), who, what);
     return v;
+}
+// what at::empty gives, without its way through the dispatcher
+at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, int device) {
+    return at::detail::empty_cuda(sizes, type, at::Device(at::kCUDA, (c10::DeviceIndex)device), std::nullopt);
 }
 bool on(const at::Tensor& t, int device) { return t.is_cuda() && t.get_device() == device; }
 int code_of(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : -1; }
@@ -115,9 +120,8 @@ Out out_of(PyObject* o, int64_t rows, int64_t cols, int64_t bits, const char* wh
     }
     Rows r;
     r.bits = (int)bits, r.rows = (int)rows, r.cols = (int)cols, r.kp = (int)padded(cols);
-    const auto bytes = at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device);
-    r.codes = at::empty({rows, r.kp * bits / 8}, bytes);
-    r.scales = at::empty({(rows + TILE_ROWS - 1) / TILE_ROWS, r.kp / CHUNK, TILE_BYTES}, bytes);
+    r.codes = empty({rows, r.kp * bits / 8}, at::kByte, device);
+    r.scales = empty({(rows + TILE_ROWS - 1) / TILE_ROWS, r.kp / CHUNK, TILE_BYTES}, at::kByte, device);
     return Out{r, nullptr};
 }
 
@@ -167,7 +171,9 @@ PyObject* dequantize(PyObject* const* a) {
         out = tensor(a[2], who, "out must be a tensor");
     } else {
         need(THPDtype_Check(a[1]), who, "dtype must be a torch dtype");
-        out = at::empty({r.rows, r.cols}, at::TensorOptions().dtype(((THPDtype*)a[1])->scalar_type).device(at::kCUDA, device));
+        const at::ScalarType type = ((THPDtype*)a[1])->scalar_type;
+        need(type == at::kFloat || type == at::kBFloat16, who, "dtype must be float32 or bfloat16");
+        out = empty({r.rows, r.cols}, type, device);
     }
     need(code_of(out) >= 0 && out.dim() == 2 && out.size(0) == r.rows && out.size(1) == r.cols && out.stride(1) == 1 &&
          on(out, device), who, "out must be float32 or bfloat16 of the rows' shape");

@@ -161,6 +161,7 @@ template <typename T, int BITS, bool WHOLE, int AHEAD>
 __global__ void __launch_bounds__(QUANT_THREADS)
 mx_quantize_kernel(const T* x, long long ld, int rows, int k, int kp, unsigned char* codes, unsigned char* scales, int shift) {
     const Place me(shift, AHEAD);
+    pdl_launch();
     pdl_wait();
     const T* from = x + (size_t)me.row * ld;
     Unit<T, WHOLE> units[AHEAD];

@@ -121,7 +121,7 @@ def _torch_flags() -> tuple[list[str], list[str]]:
     home = os.path.dirname(torch.__file__)
     # the host compiler hides what these headers warn of behind -isystem
     return (["-isystem", os.path.join(home, "include"), "-isystem", sysconfig.get_paths()["include"]],
-            ["-L", os.path.join(home, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"])
+            ["-L", os.path.join(home, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda", "-ltorch_cuda"])
 
 
 def _digest(sources: list[str], include_dirs: list[str], module: bool = False) -> str:

@@ -60,35 +60,37 @@ class MxOps:
             self._mx_module = module
         return self._mx_module
 
-    def mx_quantize(self, x, bits=8, out=None) -> MxRows:
-        """Rows of float32 or bfloat16 (any distance between them) in the format."""
+    def _mx_begin(self) -> None:
+        """Counts a launch, behind whatever ``linear(..., may_defer=True)`` has held back."""
+        if self._pending is not None or self._pending_runs is not None:
+            self.flush()
         self.launches += 1
         self.issued += 1
+
+    def mx_quantize(self, x, bits=8, out=None) -> MxRows:
+        """Rows of float32 or bfloat16 (any distance between them) in the format."""
+        self._mx_begin()
         return self.mx.quantize(x, bits, out, self._device_index)
 
     def mx_dequantize(self, q: MxRows, dtype=torch.bfloat16, out=None):
         """The numbers that rows in the format stand for (exact in bfloat16, unless below its range)."""
-        self.launches += 1
-        self.issued += 1
+        self._mx_begin()
         return self.mx.dequantize(q, dtype, out, self._device_index)
 
     def mx_rmsnorm(self, x, weight, eps, bits=8, delta=None, out=None) -> MxRows:
         """``x += delta`` (in place; float32 rows, delta float32 or bfloat16 or none), then the rows
         ``x / sqrt(mean(x^2) + eps) * weight`` in the format.  A row is at most 32,768 elements."""
-        self.launches += 1
-        self.issued += 1
+        self._mx_begin()
         return self.mx.rmsnorm(x, weight, eps, bits, delta, out, self._device_index)
 
     def mx_linear(self, a: MxRows, w: MxRows, out, accumulate=False):
         """out (+)= a @ w.T, float32 sums; ``a`` of 8 or 4 bits, ``w`` of 4."""
-        self.launches += 1
-        self.issued += 1
+        self._mx_begin()
         return self.mx.linear(a, w, out, accumulate, self.status, self._device_index)
 
     def mx_linear_glu(self, a: MxRows, w: MxRows, cols: int, bits=8, out=None) -> MxRows:
         """``silu(a @ gate.T) * (a @ up.T)``, ``cols`` columns, in the format; ``w`` from ``mx_pack_gate_up``."""
-        self.launches += 1
-        self.issued += 1
+        self._mx_begin()
         return self.mx.linear_glu(a, w, cols, bits, out, self.status, self._device_index)
 
     # ---- weights -------------------------------------------------------------------------

@@ -206,7 +206,8 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
         } else {
             if (rank == 0) {
                 const unsigned idesc = ABITS == 4 ? scaled_idesc(BM, BN, FOUR_E2M1, FOUR_E2M1)
-                                     : GLU ? scaled_idesc(BM, BN, MIXED_E4M3, MIXED_E2M1) : scaled_idesc(BM, BN, MIXED_E2M1, MIXED_E4M3);
+                                     : GLU ? scaled_idesc(BM, BN, MIXED_E4M3, MIXED_E2M1)
+                                           : scaled_idesc(BM, BN, MIXED_E2M1, MIXED_E4M3);
                 int s = 0, local = 0;
                 unsigned phase = 0;
                 for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local) {
@@ -223,7 +224,7 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
                         const unsigned char* scales = stage_s + s * 3 * T::SCALES;
                         if (issues) {
 #pragma unroll
-                            for (int j = 0; j < CHUNKS; ++j) {          // columns of a chunk: the M side's four, the N side's eight
+                            for (int j = 0; j < CHUNKS; ++j) {          // the M side's four columns, the N side's eight
                                 if (j >= held) break;
 #pragma unroll
                                 for (int t = 0; t < 3; ++t)

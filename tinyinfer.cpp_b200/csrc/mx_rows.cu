@@ -17,6 +17,12 @@ using namespace mx;
 
 constexpr int UNIT = 8;                 // elements of a thread
 
+// The next kernel's blocks may come while these run, unless there are more of these than SMs: they would take the places of the
+// ones that wait (norm with a delta, 4,096 x 512: 6.4 us with, 5.3 without; 8 rows: a product behind starts earlier).
+__device__ __forceinline__ void launch_next_early() {
+    if ((long long)gridDim.x * gridDim.y <= 148) pdl_launch();
+}
+
 __device__ __forceinline__ void widen(const uint4& raw, float (&v)[UNIT]) {
     const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
@@ -85,10 +91,10 @@ __device__ __forceinline__ unsigned top_of(const uint4& raw) {
     return max(t & 0xffff0000u, t << 16);
 }
 
-// Codes and scales of a thread's eight elements at column c of a row, `top` their block's largest magnitude, c a multiple of 128 in the first of sixteen lanes.  A
-// whole warp calls it (shuffles under a mask that is not known when compiling cost far more), lanes with nothing to store
-// with `valid` false.  `at`, `scale_words`: where the row's codes and the scale words of its chunks begin (a row's words are
-// 512 bytes apart).
+// Codes and scales of a thread's eight elements at column c of a row, `top` their block's largest magnitude, c a multiple of
+// 128 in the first of sixteen lanes.  A whole warp calls it (shuffles under a mask that is not known when compiling cost far
+// more), lanes with nothing to store with `valid` false.  `at`, `scale_words`: where the row's codes and the scale words of its
+// chunks begin (a row's words are 512 bytes apart).
 template <int BITS>
 __device__ __forceinline__ void store_codes(const float (&v)[UNIT], unsigned top, int c, bool valid, unsigned char* at,
                                             unsigned char* scale_words) {
@@ -161,7 +167,7 @@ template <typename T, int BITS, bool WHOLE, int AHEAD>
 __global__ void __launch_bounds__(QUANT_THREADS)
 mx_quantize_kernel(const T* x, long long ld, int rows, int k, int kp, unsigned char* codes, unsigned char* scales, int shift) {
     const Place me(shift, AHEAD);
-    pdl_launch();
+    launch_next_early();
     pdl_wait();
     const T* from = x + (size_t)me.row * ld;
     Unit<T, WHOLE> units[AHEAD];
@@ -206,7 +212,7 @@ __global__ void __launch_bounds__(QUANT_THREADS)
 mx_dequantize_kernel(const unsigned char* codes, const unsigned char* scales, int rows, int k, int kp, T* out, long long ld,
                      int shift) {
     const Place me(shift, AHEAD);
-    pdl_launch();
+    launch_next_early();
     pdl_wait();
     if (me.row >= rows) return;
     const unsigned char *at = codes + (size_t)me.row * kp / (8 / BITS), *words = scales + scale_at((int)me.row, 0, kp / CHUNK);
@@ -216,7 +222,8 @@ mx_dequantize_kernel(const unsigned char* codes, const unsigned char* scales, in
     for (int u = 0; u < AHEAD; ++u) {
         const int c = (me.unit + (u << shift)) * UNIT;
         if (c < k) {
-            w[u] = BITS == 8 ? *reinterpret_cast<const uint2*>(at + c) : make_uint2(*reinterpret_cast<const unsigned*>(at + c / 2), 0);
+            w[u] = BITS == 8 ? *reinterpret_cast<const uint2*>(at + c)
+                             : make_uint2(*reinterpret_cast<const unsigned*>(at + c / 2), 0);
             s[u] = words[(size_t)(c / CHUNK) * TILE_BYTES + c / BLOCK % 4];
         }
     }
@@ -240,7 +247,7 @@ mx_dequantize_any_kernel(const unsigned char* codes, const unsigned char* scales
                          int) {
     const unsigned chunks = (unsigned)kp / CHUNK, at = (blockIdx.x * QUANT_THREADS + threadIdx.x) / 32;
     const int lane = threadIdx.x & 31;
-    pdl_launch();
+    launch_next_early();
     pdl_wait();
     if (at >= (unsigned)rows * chunks) return;
     const int row = (int)(at / chunks), c = (int)(at % chunks) * CHUNK;
@@ -250,7 +257,7 @@ mx_dequantize_any_kernel(const unsigned char* codes, const unsigned char* scales
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
         const int e = b * BLOCK + lane;
-        const unsigned code = BITS == 8 ? from[e] : from[e / 2] >> (4 * (lane & 1));      // what is above a code is its neighbour
+        const unsigned code = BITS == 8 ? from[e] : from[e / 2] >> (4 * (lane & 1));      // above a code is its neighbour
         const float v = value_of<BITS>(code) * scale_value(word >> (8 * b) & 255u);
         if (c + e < k) to[e] = from_f32<T>(v);
     }
@@ -267,7 +274,7 @@ mx_rmsnorm_kernel(float* x, long long ldx, const D* delta, long long ldd, const 
     const int row = blockIdx.x;
     float* xr = x + (size_t)row * ldx;
     float v[UNITS][UNIT];
-    pdl_launch();
+    launch_next_early();
     pdl_wait();
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) load_guarded(xr, (u * (int)blockDim.x + (int)threadIdx.x) * UNIT, k, whole_x, v[u]);
@@ -295,7 +302,8 @@ mx_rmsnorm_kernel(float* x, long long ldx, const D* delta, long long ldd, const 
         load_guarded(weight, c, k, whole_w, w);
 #pragma unroll
         for (int i = 0; i < UNIT; ++i) v[u][i] = v[u][i] * inv * w[i];
-        store_codes<BITS>(v[u], top_of(v[u]), c, c < kp, codes + (size_t)row * kp / (8 / BITS), scales + scale_at(row, 0, kp / CHUNK));
+        store_codes<BITS>(v[u], top_of(v[u]), c, c < kp, codes + (size_t)row * kp / (8 / BITS),
+                          scales + scale_at(row, 0, kp / CHUNK));
     }
 }
 
@@ -347,12 +355,15 @@ template <typename D, int BITS>
 int rmsnorm(void* x, long long ldx, const void* delta, long long ldd, const void* weight, int rows, int k, int kp, float eps,
             void* codes, void* scales, void* stream) {
     const int units = kp / UNIT;
-    // as many threads as a block may have before a thread takes a second unit: 8 x 4,096 2.40 us with one, 2.79 with two, 3.88
-    // with four; 4,096 x 8,192 67.1, 72.6, 73.9
-    const int per = units <= 1024 ? 1 : units <= 2048 ? 2 : 4;
+    // As many threads as a block may have before a thread takes a second unit (us with one, two and four, with a delta: 8 x 4,096
+    // 2.4, 2.8, 3.9; 4,096 x 8,192 66.9, 72.3, 73.7), except where many rows come without a delta: then 256 threads, so that
+    // more rows are on the way at once (4,096 x 4,096 18.9, 17.3, 17.5; 4,096 x 8,192 41.2, 38.6, 32.5; 8 x 4,096 2.0, 2.3, 2.9).
+    const int most = delta == nullptr && rows > 4 * 148 ? 256 : 1024;
+    const int per = units <= most ? 1 : units <= 2 * most ? 2 : 4;
     const int threads = ((units + per - 1) / per + 31) / 32 * 32;
     TI_REQUIRE(threads <= 1024, "mx_rmsnorm: rows of %d elements are longer than 32,768", k);
-    auto kernel = per == 1 ? mx_rmsnorm_kernel<D, BITS, 1> : per == 2 ? mx_rmsnorm_kernel<D, BITS, 2> : mx_rmsnorm_kernel<D, BITS, 4>;
+    auto kernel = per == 1 ? mx_rmsnorm_kernel<D, BITS, 1>
+                : per == 2 ? mx_rmsnorm_kernel<D, BITS, 2> : mx_rmsnorm_kernel<D, BITS, 4>;
     ti_launch_pdl(kernel, (unsigned)rows, (unsigned)threads, 0, (cudaStream_t)stream, (float*)x, ldx, (const D*)delta, ldd,
                   (const float*)weight, k, kp, eps, (unsigned char*)codes, (unsigned char*)scales, whole_rows(x, ldx, 4),
                   whole_rows(delta, ldd, sizeof(D)), whole_rows(weight, 0, 4));

@@ -133,9 +133,9 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         mbar_fence_init();
     }
     if (warp == 1) tmem_alloc(tmem_slot, T::TMEM_COLS);
-    pdl_launch();
     tc_fence_before();
     __syncthreads();
+    pdl_launch();                                             // behind the allocation: what comes early must not take its columns
     tc_fence_after();
     const unsigned tmem_base = *tmem_slot;
 

@@ -161,10 +161,10 @@ mx_gemm_pairs_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_con
                      ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
     }
-    pdl_launch();
     tc_fence_before();
     __syncthreads();
     cluster_sync();                                      // both blocks' barriers exist before any use
+    pdl_launch();                                        // behind the allocation, as in mx_gemm.cu
     tc_fence_after();
     const unsigned tmem_base = *tmem_slot;
 

@@ -19,6 +19,7 @@ to nearest even and saturate (at 6 or 448), and a block with an infinity or a Na
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -48,17 +49,13 @@ def _padded(cols: int) -> int:
 
 
 class MxOps:
-    _mx_module = None
-
-    @property
+    @functools.cached_property
     def mx(self):
         """The kernels of the microscaled format with their binding, built and loaded when first needed."""
-        if self._mx_module is None:
-            from .cuda_ops import KernelError
-            module = load_module("mx")
-            module.setup(MxRows, KernelError)
-            self._mx_module = module
-        return self._mx_module
+        from .cuda_ops import KernelError
+        module = load_module("mx")
+        module.setup(MxRows, KernelError)
+        return module
 
     def _mx_begin(self) -> None:
         """Counts a launch, behind whatever ``linear(..., may_defer=True)`` has held back."""

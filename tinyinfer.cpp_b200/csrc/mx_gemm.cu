@@ -103,6 +103,50 @@ __device__ __forceinline__ void finish_glu(const Args& p, float gate, float up, 
     if (lane == 0) p.out_scales[scale_at(tok, out_col / BLOCK, p.out_kp / CHUNK)] = (unsigned char)s;
 }
 
+// A block's share of a tile's tokens, summed over the PARTS blocks of its cluster and written.  PARTS is known when compiling, so
+// that all parts of a sum are asked for before the first is added.
+template <int PARTS, int OBITS>
+__device__ __forceinline__ void finish(const Args& p, unsigned sums, int part, int warp, int lane, int n0, int tok0, int held) {
+    if (p.mode == MODE_GLU) {
+        for (int i = warp; i < (held - part + PARTS - 1) / PARTS * 2; i += THREADS / 32) {         // (token, strip)
+            const int t = part + i / 2 * PARTS, strip = i & 1;
+            if (n0 + strip * 64 >= p.n) continue;
+            float gates[PARTS], ups[PARTS], gate = 0.0f, up = 0.0f;
+#pragma unroll
+            for (int r = 0; r < PARTS; ++r) {
+                const unsigned at = map_to_rank(sums + (t * BW + strip * 64 + lane) * 4, r);
+                gates[r] = load_cluster(at);
+                ups[r] = load_cluster(at + 32 * 4);
+            }
+#pragma unroll
+            for (int r = 0; r < PARTS; ++r) gate += gates[r], up += ups[r];
+            finish_glu<OBITS>(p, gate, up, tok0 + t, n0 / 2 + strip * 32, lane);
+        }
+        return;
+    }
+    const bool by4 = p.ldc % 4 == 0 && p.n % 4 == 0 && (uintptr_t)p.c % 16 == 0;
+    const int col = n0 + lane * 4;
+    for (int t = part + warp * PARTS; t < held; t += THREADS / 32 * PARTS) {
+        float* dst = p.c + (size_t)(tok0 + t) * p.ldc + col;
+        float4 parts[PARTS], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f), old = v;
+#pragma unroll
+        for (int r = 0; r < PARTS; ++r) parts[r] = load_cluster4(map_to_rank(sums + (t * BW + lane * 4) * 4, r));
+        if (p.mode == MODE_ACCUMULATE && by4 && col < p.n) old = __ldcg(reinterpret_cast<const float4*>(dst));
+#pragma unroll
+        for (int r = 0; r < PARTS; ++r) v.x += parts[r].x, v.y += parts[r].y, v.z += parts[r].z, v.w += parts[r].w;
+        if (by4) {
+            if (col >= p.n) continue;
+            if (p.mode == MODE_ACCUMULATE) v = make_float4(old.x + v.x, old.y + v.y, old.z + v.z, old.w + v.w);
+            *reinterpret_cast<float4*>(dst) = v;
+        } else {
+            const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (col + i < p.n) dst[i] = p.mode == MODE_ACCUMULATE ? __ldcg(dst + i) + f[i] : f[i];
+        }
+    }
+}
+
 template <int NTOK, int ABITS, int OBITS>
 __global__ void __launch_bounds__(THREADS)
 mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Args p) {
@@ -256,44 +300,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         const int held_tok = min(NTOK, p.m - tok0);
         const unsigned sums = smem_u32(smem);
         pdl_wait();
-        if (p.mode == MODE_GLU) {
-            // (token, strip) pairs of this block's share
-            for (int i = warp; i < (held_tok - part + p.parts - 1) / p.parts * 2; i += THREADS / 32) {
-                const int t = part + i / 2 * p.parts, strip = i & 1;
-                if (n0 + strip * 64 >= p.n) continue;
-                float gate = 0.0f, up = 0.0f;
-                for (int r = 0; r < p.parts; ++r) {
-                    const unsigned at = map_to_rank(sums + (t * BW + strip * 64 + lane) * 4, r);
-                    gate += load_cluster(at);
-                    up += load_cluster(at + 32 * 4);
-                }
-                finish_glu<OBITS>(p, gate, up, tok0 + t, n0 / 2 + strip * 32, lane);
-            }
-        } else {
-            const bool by4 = p.ldc % 4 == 0 && p.n % 4 == 0 && (uintptr_t)p.c % 16 == 0;
-            for (int t = part + warp * p.parts; t < held_tok; t += THREADS / 32 * p.parts) {
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int r = 0; r < p.parts; ++r) {
-                    const float4 o = load_cluster4(map_to_rank(sums + (t * BW + lane * 4) * 4, r));
-                    v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-                }
-                const int col = n0 + lane * 4;
-                float* dst = p.c + (size_t)(tok0 + t) * p.ldc + col;
-                if (by4) {
-                    if (col >= p.n) continue;
-                    if (p.mode == MODE_ACCUMULATE) {
-                        const float4 o = __ldcg(reinterpret_cast<const float4*>(dst));
-                        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-                    }
-                    *reinterpret_cast<float4*>(dst) = v;
-                } else {
-                    const float f[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (col + i < p.n) dst[i] = (p.mode == MODE_ACCUMULATE ? __ldcg(dst + i) : 0.0f) + f[i];
-                }
-            }
-        }
+        if (p.parts == 8) finish<8, OBITS>(p, sums, part, warp, lane, n0, tok0, held_tok);
+        else if (p.parts == 4) finish<4, OBITS>(p, sums, part, warp, lane, n0, tok0, held_tok);
+        else if (p.parts == 2) finish<2, OBITS>(p, sums, part, warp, lane, n0, tok0, held_tok);
+        else finish<1, OBITS>(p, sums, part, warp, lane, n0, tok0, held_tok);
         cluster_sync();                                       // nobody leaves while its sums may be read
     } else {
         __syncthreads();

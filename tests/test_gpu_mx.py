@@ -187,6 +187,46 @@ def test_linear(ops, bits, m, n, k):
     assert (room[:, :2] == 3).all() and (room[:, 2 + n:] == 3).all()
 
 
+# enough tiles of 256 x 256 for pairs of SMs, none of them whole in every direction
+MANY = [(1100, 2117, 300), (2600, 1001, 129), (700, 4000, 1100), (300, 5121, 256), (129, 10400, 40)]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("m, n, k", MANY)
+def test_linear_of_many_tiles(ops, bits, m, n, k):
+    a, w = ops.mx_quantize(activations(m, m, k), bits), ops.mx_pack_linear(torch.randn(n, k, device="cuda", generator=gen(n)))
+    av, wv = mx_util.values_of(a), mx_util.values_of(w)
+    exact, tol = av @ wv.T, bound(av, wv, k)
+    room = torch.full((m + 2, n + 5), 3.0, device="cuda")
+    out = room[1:1 + m, 2:2 + n]
+    for add in (False, True):
+        old = out.double().cpu().numpy()
+        ops.mx_linear(a, w, out, accumulate=add)
+        fine(ops)
+        want = exact + old if add else exact
+        assert (np.abs(out.double().cpu().numpy() - want) <= tol + 2.0 ** -23 * np.abs(want)).all()
+    first = out.clone()
+    ops.mx_linear(a, w, out)
+    assert torch.equal(ops.mx_linear(a, w, out, accumulate=True), first)             # the same bits again
+    assert (room[[0, -1]] == 3).all() and (room[:, :2] == 3).all() and (room[:, 2 + n:] == 3).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("m, n", [(1100, 2117), (300, 200)])
+def test_products_of_many_rows_keep_nan_in_its_row_and_column(ops, bits, m, n):
+    x, w = activations(1, m, 300), torch.randn(n, 300, device="cuda", generator=gen(2))
+    x[m - 1, 290] = float("nan")
+    w[150, 3] = float("inf")
+    a = ops.mx_quantize(x, bits)
+    bad = ops.mx_linear(a, ops.mx_pack_linear(w), torch.empty(m, n, device="cuda")).isnan()
+    assert bad[m - 1].all() and bad[:, 150].all() and bad.sum() == n + m - 1
+    # gated rows: a NaN takes its block of 32 columns along, and in the row of NaN all of them
+    q = ops.mx_dequantize(ops.mx_linear_glu(a, ops.mx_pack_gate_up(w, torch.ones_like(w)), n))
+    fine(ops)
+    bad = q.isnan()
+    assert bad[m - 1].all() and bad[:, 128:160].all() and bad.sum() == n + 32 * (m - 1)
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("m", [3, 40, 300])
 def test_linear_keeps_nan_in_its_row_and_column(ops, bits, m):
@@ -307,6 +347,16 @@ def test_on_a_stream_of_its_own_and_in_a_graph(ops):
     fine(ops)
 
 
+def test_one_row_for_all(ops):
+    """Rows that share their memory may be read: a delta that is one row, an input that is."""
+    x, one = activations(1, 6, 160), activations(2, 1, 160)
+    y = x.clone()
+    got = ops.mx_dequantize(ops.mx_rmsnorm(x, torch.ones(160, device="cuda"), 1e-6, delta=one.expand(6, 160)))
+    want = ops.mx_dequantize(ops.mx_rmsnorm(y, torch.ones(160, device="cuda"), 1e-6, delta=one.repeat(6, 1)))
+    assert torch.equal(got, want) and torch.equal(x, y)
+    same_format(ops.mx_quantize(one.expand(6, 160), 4), one.repeat(6, 1))
+
+
 def test_held_back_products_run_first(ops):
     """A product that another part let the kernel set hold back is in the residual before the norm reads it."""
     from tinyinfer_b200.kernels import CudaOps
@@ -353,6 +403,7 @@ def test_refusals(ops):
         lambda: ops.mx_linear(a, a, out), lambda: ops.mx_linear(a, ops.mx_pack_linear(torch.randn(8, 65, device="cuda")), out),
         lambda: ops.mx_linear(a, w, out.bfloat16()), lambda: ops.mx_linear(a, w, out.T), lambda: ops.mx_linear(a, w, out[:3]),
         lambda: ops.mx_linear(a, w, out[:1].expand(4, 8)), lambda: ops.mx_linear(a, w, out.cpu()),
+        lambda: ops.mx_rmsnorm(x[:1].expand(4, 64), ones, 1e-6, delta=x), lambda: ops.mx_dequantize(a, out=x[:1].expand(4, 64)),
         lambda: ops.mx_linear_glu(a, w, 8), lambda: ops.mx_linear_glu(a, glu, 129), lambda: ops.mx_linear_glu(a, glu, 0),
         lambda: ops.mx_linear_glu(a, glu, 8, 3), lambda: ops.mx_linear_glu(a, glu, 8, 8, out=a),
         lambda: ops.mx_pack_gate_up(torch.randn(8, 64, device="cuda"), torch.randn(9, 64, device="cuda")),

@@ -58,6 +58,8 @@ at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, int device) {
     return at::detail::empty_cuda(sizes, type, at::Device(at::kCUDA, (c10::DeviceIndex)device), std::nullopt);
 }
 bool on(const at::Tensor& t, int device) { return t.is_cuda() && t.get_device() == device; }
+// rows that a kernel writes: none of them on another's place
+bool apart(const at::Tensor& t) { return t.size(0) <= 1 || t.stride(0) >= t.size(1); }
 int code_of(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : -1; }
 
 Rows rows_of(PyObject* o, const char* who, int device) {
@@ -177,6 +179,7 @@ PyObject* dequantize(PyObject* const* a) {
     }
     need(code_of(out) >= 0 && out.dim() == 2 && out.size(0) == r.rows && out.size(1) == r.cols && out.stride(1) == 1 &&
          on(out, device), who, "out must be float32 or bfloat16 of the rows' shape");
+    need(apart(out), who, "the rows of out must not overlap");
     if (r.rows)
         launched(ti_mx_dequantize(r.codes.data_ptr(), r.scales.data_ptr(), r.rows, r.cols, r.kp, r.bits, out.data_ptr(),
                                   code_of(out), out.stride(0), stream_of(device)));
@@ -201,6 +204,7 @@ PyObject* rmsnorm(PyObject* const* a) {
         const at::Tensor& d = tensor(a[4], who, "delta must be a tensor");
         need(d.dim() == 2 && d.sizes() == x.sizes() && d.stride(1) == 1 && code_of(d) >= 0 && on(d, device), who,
              "delta must be float32 or bfloat16 of x's shape");
+        need(apart(x), who, "the rows of x must not overlap where delta is added to them");
         delta = d.data_ptr(), delta_code = code_of(d), delta_ld = d.stride(0);
     }
     const Out out = out_of(a[5], x.size(0), x.size(1), number(a[3], who, "bits must be a whole number"), who, device);
@@ -221,7 +225,7 @@ PyObject* linear(PyObject* const* a) {
     need(out.dim() == 2 && out.size(0) == x.rows && out.size(1) == w.rows && out.stride(1) == 1 &&
          out.scalar_type() == at::kFloat && on(out, device), who, "out must be float32 of rows x weights");
     const int64_t ld = out.size(0) > 1 ? out.stride(0) : out.size(1);
-    need(ld >= out.size(1) && ld < (1LL << 31), who, "the rows of out must not overlap");
+    need(apart(out) && ld < (1LL << 31), who, "the rows of out must not overlap and lie less than 2^31 floats apart");
     if (x.rows && w.rows)
         launched(ti_mx_gemm(x.codes.data_ptr(), x.scales.data_ptr(), x.bits, w.codes.data_ptr(), w.scales.data_ptr(),
                             (float*)out.data_ptr(), x.rows, w.rows, x.kp, (int)ld, PyObject_IsTrue(a[3]) == 1, w.settled,

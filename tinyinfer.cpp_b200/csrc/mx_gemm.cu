@@ -362,13 +362,14 @@ template <int ABITS, int OBITS> int launch_rows(const void* w, const void* x, co
          : p.m <= 64 ? launch<64, ABITS, OBITS>(w, x, p, stream) : launch<128, ABITS, OBITS>(w, x, p, stream);
 }
 
-// Whether a product runs on pairs of SMs (mx_gemm_pairs.cu): with tiles of 256 x 256 for most of the 74 pairs, or where K is
-// too short to be cut.  Blocks of one SM win where their parts of K fill the GPU.  us, one SM / pairs: 512 x 4,096 x 12,288
-// (32 tiles) 30.9 / 39.1, 768 rows (48) 46.8 / 41.0, 512 x 6,144 x 4,096 (48) 19.3 / 18.0, 256 x 1,024 x 4,096 (4) 8.6 / 10.4,
-// 256 x 2,048 x 1,024 (8) 9.7 / 7.4, 1,024 x 2,048 x 512 (32) 9.9 / 6.5.  The gated form of one SM finishes many rows more
-// slowly: 128 x 2 x 12,288 x 4,096 27.3 / 18.5, 64 rows 23.4 / 27.8, 128 x 2 x 4,096 x 4,096 (32) 13.7 / 15.6.
-bool use_pairs(int m, int n, int kp, int from) {
-    return m > from && ((m + 255) / 256 * ((n + 255) / 256) >= 40 || kp <= 1024);
+// Whether a product runs on pairs of SMs (mx_gemm_pairs.cu): with tiles of 256 x 256 for most of the 74 pairs.  Below that, blocks
+// of one SM fill the GPU with their parts of K.  us, one SM / pairs: 512 x 4,096 x 12,288 (32 tiles) 28.5 / 34.5, 768 rows (48)
+// 55.1 / 35.9, 512 x 6,144 x 4,096 (48) 23.2 / 16.4, 256 x 1,024 x 4,096 (4) 6.1 / 9.3, 1,024 x 2,048 x 512 (32) 5.1 / 6.3.  The
+// gated form of one SM finishes many rows more slowly: 100 x 2 x 12,288 x 4,096 (96) 33.9 / 24.6, 64 rows 19.7 / 23.8; 200 x 2 x
+// 4,096 x 4,096 (32) 18.1 / 14.3, 128 rows 12.4 / 14.2; 512 x 2 x 1,024 x 1,024 (16) 9.6 / 7.0, x 4,096 12.4 / 13.9.
+bool use_pairs(int m, int n, int kp, bool glu) {
+    const int tiles = (m + 255) / 256 * ((n + 255) / 256);
+    return glu ? (m > 64 && tiles >= 40) || (m > 128 && (tiles >= 24 || kp <= 1024)) : m > 128 && tiles >= 40;
 }
 
 int check(const char* who, const void* a, const void* a_scales, int a_bits, const void* w, const void* w_scales, int m, int n,
@@ -388,7 +389,7 @@ extern "C" int ti_mx_gemm(const void* a, const void* a_scales, int a_bits, const
     if (int rc = check("mx_gemm", a, a_scales, a_bits, w, w_scales, m, n, kp)) return rc;
     TI_REQUIRE((uintptr_t)c % 4 == 0 && ldc >= n, "mx_gemm: rows of %d floats for %d columns", ldc, n);
     if (m == 0 || n == 0) return 0;
-    if (use_pairs(m, n, kp, 128))
+    if (use_pairs(m, n, kp, false))
         return mx_gemm_pairs(a, a_scales, a_bits, w, w_scales, c, m, n, kp, ldc, accumulate, settled, status, stream);
     const Args p{(const unsigned char*)w_scales, (const unsigned char*)a_scales, c, nullptr, nullptr, m, n, kp, ldc, 0,
                  accumulate ? MODE_ACCUMULATE : MODE_STORE, 1, 0, settled, status};
@@ -402,7 +403,7 @@ extern "C" int ti_mx_gemm_glu(const void* a, const void* a_scales, int a_bits, c
     TI_REQUIRE(out_bits == 4 || out_bits == 8, "mx_gemm_glu: output of %d bits (4 and 8 are known)", out_bits);
     TI_REQUIRE(out_kp % CHUNK == 0, "mx_gemm_glu: %d output columns are not whole chunks of 128", out_kp);
     if (m == 0 || out_kp == 0) return 0;
-    if (use_pairs(m, 2 * out_kp, kp, 64))
+    if (use_pairs(m, 2 * out_kp, kp, true))
         return mx_gemm_pairs_glu(a, a_scales, a_bits, w, w_scales, codes, scales, out_bits, m, out_kp, kp, settled, status,
                                  stream);
     const Args p{(const unsigned char*)w_scales, (const unsigned char*)a_scales, nullptr, (unsigned char*)codes,

@@ -7,9 +7,11 @@
 // is TMA's), with the scale tiles of those elements beside it.  The MMA warp copies a stage's scale tiles into tensor memory
 // columns of that stage; columns are written again when the stage's "empty" barrier has seen the products that read them.
 //
-// Bound by TMA: a block takes 0.25 us a stage whether it has 5 stages in flight or 11, with 8 KB of 4-bit weights in a stage
-// that spreads them and 16 KB in one that does not, so one request's 151,936 x 4,096 runs at 5.4 and 5.9 TB/s; for few tiles by
-// the latency of a stage and of the launch (1 x 1,024 x 1,024 3.0 us).
+// Bound by memory, through the bytes that are asked for at a time: spread codes leave half of a stage's shared memory empty, so an
+// SM holds 64 to 96 KB of W in flight.  8 rows x 2 x 12,288 x 4,096 take 12.3 us (4.4 TB/s), and some 3 of them go by before the
+// first product and behind the last; 1 x 151,936 x 4,096 runs at 6.2 TB/s, with A of 4 bits at 6.5.  Asking ahead into L2, copies
+// by threads instead of TMA for all or part of W, and other promotions in L2 were all slower.  For few tiles the latency of a
+// stage and of the launch bounds it (1 x 1,024 x 1,024 3.2 us).
 //
 // K is cut over the blocks of a cluster: each keeps its part of the sum in its shared memory, and after a cluster barrier
 // every block adds the parts of its share of the tokens, in the order of the blocks (no atomics: the same bits each run).
@@ -35,22 +37,23 @@ constexpr int ROW = 128;                     // bytes of an operand row in a sta
 enum { MODE_STORE = 0, MODE_ACCUMULATE = 1, MODE_GLU = 2 };
 enum { TI_ERR_TIMEOUT = 2 };
 
-template <int NTOK, int ABITS> struct Tile {
+template <int NTOK, int ABITS, int PER_SM> struct Tile {                 // PER_SM: blocks of an SM
     static constexpr int ELEMS = ABITS == 4 ? 256 : 128;                 // of K in a stage
     static constexpr int CHUNKS = ELEMS / CHUNK;
     static constexpr int STAGE_W = BW * ROW, STAGE_X = NTOK * ROW, STAGE_S = CHUNKS * 2 * TILE_BYTES;
-    // blocks of an SM, stages of a block's ring: two short rings for few rows (8 x 4,096 x 12,288 7.7 us, one of 11 stages 9.3),
-    // one long one where a stage is large (128 x 4,096 x 12,288 14.7 us with two of three stages, 12.9 with one of six)
-    static constexpr int PER_SM = NTOK == 128 ? 1 : 2;
-    static constexpr int STAGES = NTOK == 128 ? 6 : NTOK == 64 ? 4 : 5;
-    static constexpr int SMEM = STAGES * (STAGE_W + STAGE_X + STAGE_S) + 1024 + 256;
+    // As many stages as fit; 1,024 bytes of a block are the system's, 1,280 alignment and barriers.  Two rings an SM are better than
+    // one of the same stages where these are small (8 x 4,096 x 12,288 7.7 us, one of 11 stages 9.3), one is where they are large
+    // (128 x 4,096 x 12,288 14.7 us with two of three stages, 12.9 with one of six).
+    static constexpr int STAGES = (228 * 1024 / PER_SM - 1024 - 1280) / (STAGE_W + STAGE_X + STAGE_S);
+    static constexpr int SMEM = STAGES * (STAGE_W + STAGE_X + STAGE_S) + 1280;
     static constexpr int SCALE_COLS = CHUNKS * 8;                         // tensor memory columns of a stage's scales
     static constexpr int ACC_COLS = NTOK < 32 ? 32 : NTOK;
     static constexpr int COLS = ACC_COLS + STAGES * SCALE_COLS;
     static constexpr unsigned TMEM_COLS = COLS <= 128 ? 128 : 256;
-    static_assert(COLS <= 256, "tensor memory");
-    static_assert(SMEM * PER_SM <= 227 * 1024, "shared memory");
-    static_assert(STAGES * (STAGE_W + STAGE_X) >= NTOK * BW * 4, "the sums of a tile have to fit where the stages were");
+    static_assert(COLS <= 256 && TMEM_COLS * PER_SM <= 512, "tensor memory");
+    static_assert(STAGES >= 3, "shared memory");
+    static_assert(STAGES * (STAGE_W + STAGE_X) >= (NTOK < 16 ? 16 : NTOK) * BW * 4,
+                  "the sums of a tile have to fit where the stages were");
 };
 
 struct Args {
@@ -151,10 +154,10 @@ __device__ __forceinline__ void finish(const Args& p, unsigned sums, int part, i
     }
 }
 
-template <int NTOK, int ABITS, int OBITS>
-__global__ void __launch_bounds__(MORE_THREADS)
+template <int NTOK, int ABITS, int OBITS, int PER_SM>
+__global__ void __launch_bounds__(MORE_THREADS, PER_SM)
 mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Args p) {
-    using T = Tile<NTOK, ABITS>;
+    using T = Tile<NTOK, ABITS, PER_SM>;
     constexpr int STAGES = T::STAGES, CHUNKS = T::CHUNKS;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -305,6 +308,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         const unsigned sums = smem_u32(smem);
         pdl_wait();
         if (p.parts == 8) finish<8, OBITS>(p, sums, part, warp, lane, n0, tok0, held_tok);
+        else if (p.parts == 6) finish<6, OBITS>(p, sums, part, warp, lane, n0, tok0, held_tok);
         else if (p.parts == 4) finish<4, OBITS>(p, sums, part, warp, lane, n0, tok0, held_tok);
         else if (p.parts == 2) finish<2, OBITS>(p, sums, part, warp, lane, n0, tok0, held_tok);
         else finish<1, OBITS>(p, sums, part, warp, lane, n0, tok0, held_tok);
@@ -318,10 +322,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     }
 }
 
-template <int NTOK, int ABITS, int OBITS>
-int launch(const void* w, const void* x, Args p, void* stream) {
-    using T = Tile<NTOK, ABITS>;
-    auto kernel = mx_gemm_kernel<NTOK, ABITS, OBITS>;
+template <int NTOK, int ABITS, int OBITS, int PER_SM>
+int launch(const void* w, const void* x, const Args& p, void* stream) {
+    using T = Tile<NTOK, ABITS, PER_SM>;
+    auto kernel = mx_gemm_kernel<NTOK, ABITS, OBITS, PER_SM>;
     CUtensorMap map_w, map_x;
     if (int rc = make_map_codes(&map_w, w, p.n, p.kp, 4, ABITS == 8, BW, "mx_gemm")) return rc;
     if (int rc = make_map_codes(&map_x, x, p.m, p.kp, ABITS, false, NTOK, "mx_gemm")) return rc;
@@ -331,17 +335,8 @@ int launch(const void* w, const void* x, Args p, void* stream) {
         if (e != cudaSuccess) return ti_fail("mx_gemm: %s", cudaGetErrorString(e));
         configured.mark();
     }
-    int device = 0, sms = 0;
-    cudaGetDevice(&device);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    p.tiles_n = (p.n + BW - 1) / BW;
-    const int tiles = p.tiles_n * ((p.m + NTOK - 1) / NTOK), num_kb = (p.kp + T::ELEMS - 1) / T::ELEMS;
-    // K in as many parts as find blocks at once (two an SM), in 8 only where a part is long enough to be worth the larger
-    // cluster: us with 4 / 8 parts, 8 rows x 4,096 x 4,096 (32 stages) 4.9 / 5.8, 8 x 4,096 x 12,288 (96) 9.0 / 7.9
-    p.parts = 1;
-    while (p.parts < (num_kb >= 40 ? 8 : 4) && tiles * p.parts * 2 <= sms * T::PER_SM && p.parts * 2 <= num_kb) p.parts *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = (unsigned)(tiles * p.parts);
+    cfg.gridDim = (unsigned)(p.tiles_n * ((p.m + NTOK - 1) / NTOK) * p.parts);
     cfg.blockDim = p.mode == MODE_GLU || NTOK == 128 ? MORE_THREADS : THREADS;
     cfg.dynamicSmemBytes = T::SMEM;
     cfg.stream = (cudaStream_t)stream;
@@ -353,13 +348,65 @@ int launch(const void* w, const void* x, Args p, void* stream) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, (const Args)p);
+    cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, p);
     return ti_check_launch("mx_gemm");
 }
 
-template <int ABITS, int OBITS> int launch_rows(const void* w, const void* x, const Args& p, void* stream) {
-    return p.m <= 16 ? launch<16, ABITS, OBITS>(w, x, p, stream) : p.m <= 32 ? launch<32, ABITS, OBITS>(w, x, p, stream)
-         : p.m <= 64 ? launch<64, ABITS, OBITS>(w, x, p, stream) : launch<128, ABITS, OBITS>(w, x, p, stream);
+// Into how many parts K is cut (blocks of a cluster), and how many blocks an SM takes, for tiles of `per` blocks an SM, or of up
+// to 32 rows (per 0), which have a long ring for two blocks of an SM and a short one for three.  steps: stages of a tile.  Figures
+// are us for 8 rows of 8 bits.
+struct Split {
+    int parts, per_sm;
+};
+
+Split split(int tiles, int steps, bool glu, int per) {
+    // The blocks of a cluster lie in one group of SMs: of 148, clusters of 4 and 6 reach 132 and clusters of 8 120.  More clusters
+    // than lie there at once make a second wave: 32 tiles of K = 12,288 in 8 / 6 parts 7.8 / 7.5, 44 tiles 13.9 / 9.0.
+    const auto fits = [&](int parts, int blocks) { return tiles * parts <= (parts <= 2 ? 148 : parts <= 6 ? 132 : 120) * blocks; };
+    // A part has to be worth its exchange of sums: with 1 / 2 / 4 parts, 32 tiles of K = 1,024 3.3 / 3.7 / 3.7, of 1,536 4.1 / 4.2 /
+    // 4.0, of 4,096 8.9 / 6.1 / 4.6 (with 8 5.8); 80 tiles of 2,048 5.17 / 5.18, of 2,816 6.6 / 5.6.  A gated tile is finished by
+    // more warps when cut: of 512 with 1 / 2, 64 tiles 4.0 / 3.7, of 1,024 with 1 / 2 / 4 16 tiles 4.4 / 3.5 / 3.5; 64 rows, 44
+    // tiles of 1,024 with 2 / 4 6.8 / 6.2, 16 of 512 5.8 / 5.1.
+    const auto worth = [&](int parts) {
+        if (parts > 4) return steps >= 8 * parts;
+        if (parts == 2) return steps >= (glu ? 4 : 20);
+        if (glu && per) return steps >= 4;
+        return steps >= (!fits(4, 1) ? 16 : glu ? 8 : 12);
+    };
+    const auto most = [&](int blocks) {
+        for (int parts : {8, 6, 4, 2})
+            if (fits(parts, blocks) && worth(parts)) return parts;
+        return 1;
+    };
+    if (per) return {most(per), per};
+    // Three blocks where two do not take all tiles at once (two / three: 400 tiles of 4,096 25.1 / 19.8, 296 of 1,024 4.8 / 4.2),
+    // where they make room for two parts (gated, 192 tiles of 4,096, 14.0 / 12.3) or four (72 tiles of 12,288 15.4 / 13.7), and for
+    // the room they leave the next kernel's blocks beside short parts (48 tiles of 4,096 5.5 / 5.2; 100 of 2,816 6.0 / 5.6).
+    // Elsewhere the longer ring is the better one (44 tiles of 12,288 9.0 / 10.0, 240 tiles of 4,096 in one part 13.8 / 15.7).
+    if (!fits(1, 2) || (!fits(2, 3) && steps <= 8)) return {1, 3};
+    if (!fits(2, 2)) return fits(2, 3) && steps >= (glu ? 16 : 24) ? Split{2, 3} : Split{1, 2};
+    if (steps >= 64 && !fits(4, 2) && fits(4, 3)) return {4, 3};
+    const int parts = most(2);
+    const bool narrow = (parts == 4 && !fits(4, 1) && steps < 64) || (parts == 2 && !fits(2, 1) && steps <= 24);
+    return {parts, narrow ? 3 : 2};
+}
+
+template <int ABITS, int OBITS> int launch_rows(const void* w, const void* x, Args p, void* stream) {
+    p.tiles_n = (p.n + BW - 1) / BW;
+    const int steps = (p.kp + Tile<16, ABITS, 2>::ELEMS - 1) / Tile<16, ABITS, 2>::ELEMS;
+    const bool glu = p.mode == MODE_GLU;
+    if (p.m > 32) {
+        const Split s = p.m > 64 ? split(p.tiles_n * ((p.m + 127) / 128), steps, glu, 1) : split(p.tiles_n, steps, glu, 2);
+        p.parts = s.parts;
+        return p.m > 64 ? launch<128, ABITS, OBITS, 1>(w, x, p, stream) : launch<64, ABITS, OBITS, 2>(w, x, p, stream);
+    }
+    const Split s = split(p.tiles_n, steps, glu, 0);
+    p.parts = s.parts;
+    if (s.per_sm == 3)
+        return p.m <= 8 ? launch<8, ABITS, OBITS, 3>(w, x, p, stream) : p.m <= 16 ? launch<16, ABITS, OBITS, 3>(w, x, p, stream)
+                                                                                  : launch<32, ABITS, OBITS, 3>(w, x, p, stream);
+    return p.m <= 8 ? launch<8, ABITS, OBITS, 2>(w, x, p, stream) : p.m <= 16 ? launch<16, ABITS, OBITS, 2>(w, x, p, stream)
+                                                                              : launch<32, ABITS, OBITS, 2>(w, x, p, stream);
 }
 
 // Whether a product runs on pairs of SMs (mx_gemm_pairs.cu): with tiles of 256 x 256 for most of the 74 pairs.  Below that, blocks

@@ -211,6 +211,31 @@ def test_linear_of_many_tiles(ops, bits, m, n, k):
     assert (room[[0, -1]] == 3).all() and (room[:, :2] == 3).all() and (room[:, 2 + n:] == 3).all()
 
 
+# Every number of parts of K and of blocks of an SM: tiles of 128 weight rows by stages of K (128 elements beside rows of 8
+# bits, 256 beside 4): 297 x 2, 223 x 8, 223 x 8, 149 x 25, 67 x 64, 35 x 16, 76 x 21, 32 x 48, 3 x 65, 35 x 16, 17 x 12, 9 x 9
+SPLITS = [(5, 38001, 160, 8), (8, 28500, 900, 8), (20, 28500, 900, 8), (3, 18990, 3081, 8), (9, 8500, 8103, 8), (31, 4400, 2000, 8),
+          (16, 9700, 2600, 8), (7, 4000, 6050, 8), (32, 300, 8203, 8), (8, 4401, 4000, 4), (1, 2100, 1500, 8), (2, 1100, 1100, 8),
+          (50, 4000, 6050, 8), (4, 38001, 300, 4)]
+
+
+@pytest.mark.parametrize("m, n, k, bits", SPLITS)
+def test_linear_of_every_split(ops, m, n, k, bits):
+    a, w = ops.mx_quantize(activations(m, m, k), bits), ops.mx_pack_linear(torch.randn(n, k, device="cuda", generator=gen(n)))
+    av, wv = mx_util.values_of(a), mx_util.values_of(w)
+    exact, tol = av @ wv.T, bound(av, wv, k)
+    room = torch.full((m + 2, n + 5), 3.0, device="cuda")
+    out = room[1:1 + m, 2:2 + n]
+    ops.mx_linear(a, w, out)
+    first = out.clone()
+    for add in (False, True):
+        want = exact + out.double().cpu().numpy() if add else exact
+        ops.mx_linear(a, w, out, accumulate=add)
+        fine(ops)
+        assert (np.abs(out.double().cpu().numpy() - want) <= tol + 2.0 ** -23 * np.abs(want)).all()
+        assert add or torch.equal(out, first)                                        # the same bits again
+    assert (room[[0, -1]] == 3).all() and (room[:, :2] == 3).all() and (room[:, 2 + n:] == 3).all()
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("m, n", [(1100, 2117), (300, 200)])
 def test_products_of_many_rows_keep_nan_in_its_row_and_column(ops, bits, m, n):
@@ -295,6 +320,13 @@ def test_glu(ops, obits, bits, m, n, k):
     assert (off <= mx_util.rounding(np.abs(exact) + off_by, obits) + off_by).all()
     codes, scales = mx_util.unpack(q)
     assert not codes[:, n:].any() and (scales != 255).all()
+
+
+# tiles by stages 149 x 16, 297 x 2, 35 x 16, 80 x 21, 17 x 8, 6 x 50, 17 x 4
+@pytest.mark.parametrize("m, n, k", [(3, 9520, 2000), (8, 18960, 200), (10, 2200, 2000), (30, 5100, 2600), (6, 1030, 1000),
+                                     (9, 380, 6300), (60, 1030, 500)])
+def test_glu_of_every_split(ops, m, n, k):
+    test_glu(ops, 8, 8, m, n, k)
 
 
 @pytest.mark.parametrize("m", [3, 300])

@@ -379,16 +379,15 @@ Split split(int tiles, int steps, bool glu, int per) {
         return 1;
     };
     if (per) return {most(per), per};
-    // Three blocks where two do not take all tiles at once (two / three: 400 tiles of 4,096 25.1 / 19.8, 296 of 1,024 4.8 / 4.2),
-    // where they make room for two parts (gated, 192 tiles of 4,096, 14.0 / 12.3) or four (72 tiles of 12,288 15.4 / 13.7), and for
-    // the room they leave the next kernel's blocks beside short parts (48 tiles of 4,096 5.5 / 5.2; 100 of 2,816 6.0 / 5.6).
-    // Elsewhere the longer ring is the better one (44 tiles of 12,288 9.0 / 10.0, 240 tiles of 4,096 in one part 13.8 / 15.7).
-    if (!fits(1, 2) || (!fits(2, 3) && steps <= 8)) return {1, 3};
+    // Three blocks where two do not take all tiles at once (two / three: 400 tiles of 4,096 25.1 / 19.8), where they make room for
+    // two parts (gated, 192 tiles of 4,096, 14.0 / 12.3; tiles of 2,048 6.1 in one part, 7.3) or four (behind a norm of the rows,
+    // that included, 80 tiles of 4,096 8.4 / 7.8, 72 of 12,288 18.7 / 16.7; 99 of 2,816 7.2 / 7.4).  Elsewhere the longer ring is
+    // the better one (44 tiles of 12,288 9.0 / 10.0, 240 tiles of 4,096 in one part 13.8 / 15.7; behind a norm, 48 of 4,096 6.8 /
+    // 6.9, though one behind another of its like they take 5.5 / 5.2).
+    if (!fits(1, 2)) return {1, 3};
     if (!fits(2, 2)) return fits(2, 3) && steps >= (glu ? 16 : 24) ? Split{2, 3} : Split{1, 2};
-    if (steps >= 64 && !fits(4, 2) && fits(4, 3)) return {4, 3};
-    const int parts = most(2);
-    const bool narrow = (parts == 4 && !fits(4, 1) && steps < 64) || (parts == 2 && !fits(2, 1) && steps <= 24);
-    return {parts, narrow ? 3 : 2};
+    if (steps >= 32 && !fits(4, 2) && fits(4, 3)) return {4, 3};
+    return {most(2), 2};
 }
 
 template <int ABITS, int OBITS> int launch_rows(const void* w, const void* x, Args p, void* stream) {

@@ -7,11 +7,11 @@
 // is TMA's), with the scale tiles of those elements beside it.  The MMA warp copies a stage's scale tiles into tensor memory
 // columns of that stage; columns are written again when the stage's "empty" barrier has seen the products that read them.
 //
-// Bound by memory, through the bytes that are asked for at a time: spread codes leave half of a stage's shared memory empty, so an
-// SM holds 64 to 96 KB of W in flight.  8 rows x 2 x 12,288 x 4,096 take 12.3 us (4.4 TB/s), and some 3 of them go by before the
-// first product and behind the last; 1 x 151,936 x 4,096 runs at 6.2 TB/s, with A of 4 bits at 6.5.  Asking ahead into L2, copies
-// by threads instead of TMA for all or part of W, and other promotions in L2 were all slower.  For few tiles the latency of a
-// stage and of the launch bounds it (1 x 1,024 x 1,024 3.2 us).
+// Bound by memory, through the bytes that are asked for at a time: spread codes leave half of a stage's shared memory empty, so
+// an SM holds 64 to 96 KB of W in flight.  8 rows x 2 x 12,288 x 4,096 take 12.3 us (4.4 TB/s), and some 3 of them go by before
+// the first product and behind the last; 1 x 151,936 x 4,096 runs at 6.2 TB/s, with A of 4 bits at 6.5.  Asking ahead into L2,
+// copies by threads instead of TMA for all or part of W, and other promotions in L2 were all slower.  For few tiles the latency
+// of a stage and of the launch bounds it (1 x 1,024 x 1,024 3.2 us).
 //
 // K is cut over the blocks of a cluster: each keeps its part of the sum in its shared memory, and after a cluster barrier
 // every block adds the parts of its share of the tokens, in the order of the blocks (no atomics: the same bits each run).
@@ -41,9 +41,9 @@ template <int NTOK, int ABITS, int PER_SM> struct Tile {                 // PER_
     static constexpr int ELEMS = ABITS == 4 ? 256 : 128;                 // of K in a stage
     static constexpr int CHUNKS = ELEMS / CHUNK;
     static constexpr int STAGE_W = BW * ROW, STAGE_X = NTOK * ROW, STAGE_S = CHUNKS * 2 * TILE_BYTES;
-    // As many stages as fit; 1,024 bytes of a block are the system's, 1,280 alignment and barriers.  Two rings an SM are better than
-    // one of the same stages where these are small (8 x 4,096 x 12,288 7.7 us, one of 11 stages 9.3), one is where they are large
-    // (128 x 4,096 x 12,288 14.7 us with two of three stages, 12.9 with one of six).
+    // As many stages as fit; 1,024 bytes of a block are the system's, 1,280 alignment and barriers.  Two rings an SM are better
+    // than one of the same stages where these are small (8 x 4,096 x 12,288 7.7 us, one of 11 stages 9.3), one is where they
+    // are large (128 x 4,096 x 12,288 14.7 us with two of three stages, 12.9 with one of six).
     static constexpr int STAGES = (228 * 1024 / PER_SM - 1024 - 1280) / (STAGE_W + STAGE_X + STAGE_S);
     static constexpr int SMEM = STAGES * (STAGE_W + STAGE_X + STAGE_S) + 1280;
     static constexpr int SCALE_COLS = CHUNKS * 8;                         // tensor memory columns of a stage's scales
@@ -352,26 +352,29 @@ int launch(const void* w, const void* x, const Args& p, void* stream) {
     return ti_check_launch("mx_gemm");
 }
 
-// Into how many parts K is cut (blocks of a cluster), and how many blocks an SM takes, for tiles of `per` blocks an SM, or of up
-// to 32 rows (per 0), which have a long ring for two blocks of an SM and a short one for three.  steps: stages of a tile.  Figures
-// are us for 8 rows of 8 bits.
+// Into how many parts K is cut (blocks of a cluster), and how many blocks an SM takes, for tiles of `per` blocks an SM, or of
+// up to 32 rows (per 0), which have a long ring for two blocks of an SM and a short one for three.  steps: stages of a tile.
+// Figures are us for 8 rows of 8 bits.
 struct Split {
     int parts, per_sm;
 };
 
 Split split(int tiles, int steps, bool glu, int per) {
-    // The blocks of a cluster lie in one group of SMs: of 148, clusters of 4 and 6 reach 132 and clusters of 8 120.  More clusters
-    // than lie there at once make a second wave: 32 tiles of K = 12,288 in 8 / 6 parts 7.8 / 7.5, 44 tiles 13.9 / 9.0.
+    // The blocks of a cluster lie in one group of SMs: of 148, clusters of 4 and 6 reach 132 and clusters of 8 120.  More
+    // clusters than lie there at once make a second wave: 32 tiles of K = 12,288 in 8 / 6 parts 7.8 / 7.5, 44 tiles 13.9 / 9.0.
     const auto fits = [&](int parts, int blocks) { return tiles * parts <= (parts <= 2 ? 148 : parts <= 6 ? 132 : 120) * blocks; };
-    // A part has to be worth its exchange of sums: with 1 / 2 / 4 parts, 32 tiles of K = 1,024 3.3 / 3.7 / 3.7, of 1,536 4.1 / 4.2 /
-    // 4.0, of 4,096 8.9 / 6.1 / 4.6 (with 8 5.8); 80 tiles of 2,048 5.17 / 5.18, of 2,816 6.6 / 5.6.  A gated tile is finished by
-    // more warps when cut: of 512 with 1 / 2, 64 tiles 4.0 / 3.7, of 1,024 with 1 / 2 / 4 16 tiles 4.4 / 3.5 / 3.5; 64 rows, 44
-    // tiles of 1,024 with 2 / 4 6.8 / 6.2, 16 of 512 5.8 / 5.1.
+    // A part has to be worth its exchange of sums.  With 1 / 2 / 4 parts, 32 tiles of K = 512 2.5 / 3.4 / 3.5, of 1,024 3.3 /
+    // 3.7 / 3.7 one launch behind another of its like, and in four parts 1.2 us less for a whole layer with 8 requests, whose
+    // products find their weights on the way in more SMs; of 1,536 4.1 / 4.2 / 4.0, of 4,096 8.9 / 6.1 / 4.6 (with 8 5.8; 16
+    // tiles with 4 / 8 4.5 / 4.3); 80 tiles of 2,048 5.17 / 5.18 (behind a norm and from memory 7.5 / 7.3), of 2,816 6.6 / 5.6.
+    // A gated tile is finished by more warps when cut: of 512 with 1 / 2, 64 tiles 4.0 / 3.7, of 1,024 with 1 / 2 / 4 16 tiles
+    // 4.4 / 3.5 / 3.5; 64 rows, 44 tiles of 1,024 with 2 / 4 6.8 / 6.2, 16 of 512 5.8 / 5.1.  77 rows, 5 plain tiles of 1,000
+    // with 1 / 4 4.5 / 5.0.
     const auto worth = [&](int parts) {
-        if (parts > 4) return steps >= 8 * parts;
-        if (parts == 2) return steps >= (glu ? 4 : 20);
+        if (parts > 4) return steps >= 8 * parts || (!per && parts == 8 && tiles * parts <= 148 && steps >= 24);
+        if (parts == 2) return steps >= (glu ? 4 : 16);
         if (glu && per) return steps >= 4;
-        return steps >= (!fits(4, 1) ? 16 : glu ? 8 : 12);
+        return steps >= (!glu && !fits(4, 1) ? 16 : per ? 12 : 8);
     };
     const auto most = [&](int blocks) {
         for (int parts : {8, 6, 4, 2})
@@ -379,13 +382,14 @@ Split split(int tiles, int steps, bool glu, int per) {
         return 1;
     };
     if (per) return {most(per), per};
-    // Three blocks where two do not take all tiles at once (two / three: 400 tiles of 4,096 25.1 / 19.8), where they make room for
-    // two parts (gated, 192 tiles of 4,096, 14.0 / 12.3; tiles of 2,048 6.1 in one part, 7.3) or four (behind a norm of the rows,
-    // that included, 80 tiles of 4,096 8.4 / 7.8, 72 of 12,288 18.7 / 16.7; 99 of 2,816 7.2 / 7.4).  Elsewhere the longer ring is
-    // the better one (44 tiles of 12,288 9.0 / 10.0, 240 tiles of 4,096 in one part 13.8 / 15.7; behind a norm, 48 of 4,096 6.8 /
-    // 6.9, though one behind another of its like they take 5.5 / 5.2).
+    // Three blocks where two do not take all tiles at once (two / three: 400 tiles of 4,096 25.1 / 19.8), where they make room
+    // for two parts (gated, 192 tiles of 4,096, 14.0 / 12.3, 160 of 1,024, behind a norm and from memory, 7.6 / 6.9; plain ones
+    // of 2,048 9.2 / 9.7) or four (behind a norm of the rows, that included, 80 tiles of 4,096 8.4 / 7.8, 72 of 12,288 18.7 /
+    // 16.7; 99 of 2,816 7.2 / 7.4).  Elsewhere the longer ring is the better one (44 tiles of 12,288 9.0 / 10.0, 240 tiles of
+    // 4,096 in one part 13.8 / 15.7; behind a norm, 48 of 4,096 6.8 / 6.9, though one behind another of its like they take 5.5
+    // / 5.2).
     if (!fits(1, 2)) return {1, 3};
-    if (!fits(2, 2)) return fits(2, 3) && steps >= (glu ? 16 : 24) ? Split{2, 3} : Split{1, 2};
+    if (!fits(2, 2)) return fits(2, 3) && steps >= (glu ? 8 : 20) ? Split{2, 3} : Split{1, 2};
     if (steps >= 32 && !fits(4, 2) && fits(4, 3)) return {4, 3};
     return {most(2), 2};
 }
@@ -408,11 +412,12 @@ template <int ABITS, int OBITS> int launch_rows(const void* w, const void* x, Ar
                                                                               : launch<32, ABITS, OBITS, 2>(w, x, p, stream);
 }
 
-// Whether a product runs on pairs of SMs (mx_gemm_pairs.cu): with tiles of 256 x 256 for most of the 74 pairs.  Below that, blocks
-// of one SM fill the GPU with their parts of K.  us, one SM / pairs: 512 x 4,096 x 12,288 (32 tiles) 28.5 / 34.5, 768 rows (48)
-// 55.1 / 35.9, 512 x 6,144 x 4,096 (48) 23.2 / 16.4, 256 x 1,024 x 4,096 (4) 6.1 / 9.3, 1,024 x 2,048 x 512 (32) 5.1 / 6.3.  The
-// gated form of one SM finishes many rows more slowly: 100 x 2 x 12,288 x 4,096 (96) 33.9 / 24.6, 64 rows 19.7 / 23.8; 200 x 2 x
-// 4,096 x 4,096 (32) 18.1 / 14.3, 128 rows 12.4 / 14.2; 512 x 2 x 1,024 x 1,024 (16) 9.6 / 7.0, x 4,096 12.4 / 13.9.
+// Whether a product runs on pairs of SMs (mx_gemm_pairs.cu): with tiles of 256 x 256 for most of the 74 pairs.  Below that,
+// blocks of one SM fill the GPU with their parts of K.  us, one SM / pairs: 512 x 4,096 x 12,288 (32 tiles) 28.5 / 34.5, 768
+// rows (48) 55.1 / 35.9, 512 x 6,144 x 4,096 (48) 23.2 / 16.4, 256 x 1,024 x 4,096 (4) 6.1 / 9.3, 1,024 x 2,048 x 512 (32) 5.1
+// / 6.3.  The gated form of one SM finishes many rows more slowly: 100 x 2 x 12,288 x 4,096 (96) 33.9 / 24.6, 64 rows 19.7 /
+// 23.8; 200 x 2 x 4,096 x 4,096 (32) 18.1 / 14.3, 128 rows 12.4 / 14.2; 512 x 2 x 1,024 x 1,024 (16) 9.6 / 7.0, x 4,096 12.4 /
+// 13.9.
 bool use_pairs(int m, int n, int kp, bool glu) {
     const int tiles = (m + 255) / 256 * ((n + 255) / 256);
     return glu ? (m > 64 && tiles >= 40) || (m > 128 && (tiles >= 24 || kp <= 1024)) : m > 128 && tiles >= 40;
